@@ -92,4 +92,68 @@ typedef struct DecGemmParams {
     float scale;             // QKV + attention: the score scale 1/sqrt(hd)
 } DecGemmParams;
 
+/* Paged cache (kernels/paged.hip, kernels/paged_attn.hip, host serve.c): the
+ * cache and the sequences as in trlm_serve.h, page_size as its shift */
+typedef struct PagedKv {
+    void* k;
+    void* v;
+    float* ks;               // TRLM_KV_I8: one scale for each token and head
+    float* vs;
+    const int* q_start;
+    const int* kv_len;
+    const int* pages;
+    int n, rows;
+    int num_pages, page_shift, max_pages, kv_heads;
+} PagedKv;
+
+typedef struct KvAppendParams {
+    PagedKv kv;
+    const float* q;
+    const float* k;
+    const float* v;
+    float* q_out;
+    const float* cos_t;
+    const float* sin_t;
+    int ldq, ldk, ldv, ldqo;
+    int heads;
+    int max_pos, rot, rot_half;
+} KvAppendParams;
+
+typedef struct KvReadParams {
+    PagedKv kv;
+    float* k_out;
+    float* v_out;
+    int ld;
+} KvReadParams;
+
+typedef struct PagedAttnParams {
+    PagedKv kv;
+    const float* q;
+    float* out;
+    float* part_o;           // [row][head][splits][head_dim]: a split's weighted sum, not yet divided
+    float* part_ml;          // [row][head][splits][2]: its base-2 maximum and its sum of weights
+    int ldq, ldo, heads;
+    int max_q, max_kv;
+    int splits, chunk;       // keys [s * chunk, (s + 1) * chunk) of a sequence are split s
+    float scale;
+} PagedAttnParams;
+
+/* Rules on logits (kernels/logits.hip, host serve.c) */
+typedef struct RulesParams {
+    const float* logits;
+    float* out;
+    const unsigned* history;
+    const int* hist_len;
+    const int* gen_start;
+    const float* repetition;
+    const float* frequency;
+    const float* presence;
+    const unsigned* bias_ids;
+    const float* bias;
+    const int* n_bias;
+    const unsigned* mask;
+    long long ld, ld_out, ld_hist, ld_bias, ld_mask;
+    int vocab;
+} RulesParams;
+
 #endif /* TRLM_KERNEL_PARAMS_H */

@@ -8,3 +8,6 @@
 #include "attention.hip"
 #include "decode.hip"
 #include "decode_fused.hip"
+#include "paged.hip"
+#include "paged_attn.hip"
+#include "logits.hip"

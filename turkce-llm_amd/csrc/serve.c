@@ -1,0 +1,302 @@
+/* serve.c -- host side of the serving operators (trlm_serve.h): argument
+ * checks, launch shapes, the split of long contexts. */
+#include <stdio.h>
+#include <stdlib.h>
+#include <string.h>
+#include <unistd.h>
+
+#include "trlm_serve.h"
+#include "gpu_internal.h"
+#include "kernel_params.h"
+
+#define NHD 4
+#define NTYPE 3
+static const u32 HDS[NHD] = { 16, 32, 64, 128 };
+static const char* const TYPE_NAMES[NTYPE] = { "f32", "bf16", "i8" };
+
+struct TrlmServe {
+    HipCtx* ctx;
+    i32 device;
+    /* looked up on first use of a head width and type */
+    hipFunction_t append[NHD][NTYPE][2], read[NHD][NTYPE][2], few[NHD][NTYPE], join[NHD];
+    hipFunction_t rules[2][2];   /* [narrow, wide][aligned, not] */
+};
+
+TrlmServe* trlm_serve_create(HipCtx* ctx) {
+    TrlmServe* e = (TrlmServe*)calloc(1, sizeof(TrlmServe));
+    if (!e) {
+        fprintf(stderr, "[HIP ERROR] trlm_serve_create: out of host memory\n");
+        fflush(stderr);
+        _exit(1);
+    }
+    e->ctx = ctx;
+    e->device = ctx->device;
+    return e;
+}
+
+void trlm_serve_destroy(TrlmServe* e) { free(e); }
+
+static i32 refuse(const char* op, const char* why) {
+    fprintf(stderr, "%s: refused, nothing launched: %s\n", op, why);
+    fflush(stderr);
+    return -1;
+}
+
+static int unaligned(hipDeviceptr_t p, u64 to) { return !p || ((u64)(uintptr_t)p & (to - 1)) != 0; }
+static u64 cdiv64(u64 a, u64 b) { return (a + b - 1) / b; }
+
+static i32 hd_index(u32 hd) {
+    for (i32 i = 0; i < NHD; i++)
+        if (HDS[i] == hd) return i;
+    return -1;
+}
+
+static hipFunction_t kernel(TrlmServe* e, hipFunction_t* slot, const char* name) {
+    if (!*slot) *slot = hip_get_kernel(e->ctx, name);
+    return *slot;
+}
+
+static hipFunction_t kernel_hd(TrlmServe* e, hipFunction_t* slot, const char* stem, i32 hd, i32 type) {
+    if (!*slot) {
+        char name[64];
+        if (type < 0) snprintf(name, sizeof(name), "%s_hd%u", stem, HDS[hd]);
+        else snprintf(name, sizeof(name), "%s_hd%u_%s", stem, HDS[hd], TYPE_NAMES[type]);
+        *slot = hip_get_kernel(e->ctx, name);
+    }
+    return *slot;
+}
+
+/* NULL, or why the handle cannot be used on this thread. */
+static const char* handle_fault(const TrlmServe* e) {
+    if (!e) return "no handle";
+    int cur = -1;
+    if (hipGetDevice(&cur) != hipSuccess || cur != e->device) return "the handle belongs to another device than the current one";
+    return NULL;
+}
+
+/* NULL, or what is wrong with a cache and a call's sequences. */
+static const char* cache_fault(const TrlmKvCache* c, const TrlmKvSeqs* s) {
+    if (!c || !s) return "no cache or no sequences";
+    if (c->type > TRLM_KV_I8) return "unknown cache type";
+    if (hd_index(c->head_dim) < 0) return "head_dim must be 16, 32, 64 or 128";
+    if (c->kv_heads < 1 || c->kv_heads > 1024) return "kv_heads must be 1 to 1024";
+    if (c->page_size < 16 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)))
+        return "page_size must be a power of two, 16 to 65536";
+    if (c->num_pages < 1 || c->num_pages > 0x7fffffffu) return "num_pages must be 1 to 2^31 - 1";
+    if (unaligned(c->k, 16) || unaligned(c->v, 16)) return "k and v must be 16-byte aligned device buffers";
+    if (c->type == TRLM_KV_I8 && (unaligned(c->k_scale, 16) || unaligned(c->v_scale, 16)))
+        return "an 8-bit cache needs 16-byte aligned k_scale and v_scale";
+    if (s->n > TRLM_SERVE_MAX_SEQS) return "more than 4096 sequences";
+    if (s->rows >= (1u << 24)) return "rows must be below 2^24";
+    if (s->max_pages < 1 || (u64)s->max_pages * c->page_size > (1ull << 30))
+        return "max_pages * page_size must be 1 to 2^30";
+    if (unaligned(s->q_start, 4) || unaligned(s->kv_len, 4) || unaligned(s->pages, 4))
+        return "q_start, kv_len and pages must be 4-byte aligned device buffers";
+    return NULL;
+}
+
+static u32 shift_of(u32 x) {
+    u32 s = 0;
+    while ((1u << s) < x) s++;
+    return s;
+}
+
+static PagedKv paged_kv(const TrlmKvCache* c, const TrlmKvSeqs* s) {
+    PagedKv p;
+    memset(&p, 0, sizeof(p));
+    p.k = c->k; p.v = c->v;
+    p.ks = (float*)c->k_scale; p.vs = (float*)c->v_scale;
+    p.q_start = (const int*)s->q_start; p.kv_len = (const int*)s->kv_len; p.pages = (const int*)s->pages;
+    p.n = (int)s->n; p.rows = (int)s->rows;
+    p.num_pages = (int)c->num_pages; p.page_shift = (int)shift_of(c->page_size);
+    p.max_pages = (int)s->max_pages; p.kv_heads = (int)c->kv_heads;
+    return p;
+}
+
+/* Rows a 256-thread workgroup of the append and read kernels moves per head:
+ * one per head_dim / 4 lanes, or four where that still leaves at least four
+ * workgroups for each of the 256 compute units. */
+static int four_rows(u64 rows, u32 hd, u32 heads) { return cdiv64(rows, 4 * (1024 / hd)) * heads >= 1024; }
+
+i32 trlm_kv_append(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, const TrlmKvRows* r) {
+    static const char* op = "trlm_kv_append";
+    const char* why = handle_fault(e);
+    if (!why) why = cache_fault(c, s);
+    if (why) return refuse(op, why);
+    if (!r) return refuse(op, "no rows");
+    const u32 hd = c->head_dim;
+    if (unaligned(r->k, 16) || unaligned(r->v, 16) || (r->ldk | r->ldv) % 4)
+        return refuse(op, "k and v rows must be 16-byte aligned");
+    if (r->ldk < c->kv_heads * hd || r->ldv < c->kv_heads * hd || (r->ldk | r->ldv) > 0x7fffffffu)
+        return refuse(op, "ldk and ldv must hold a row");
+    if (!r->q != !r->heads || !r->q != !r->q_out) return refuse(op, "q, q_out and heads go together");
+    if (r->heads > 1024) return refuse(op, "more than 1024 heads");
+    if (r->heads && (unaligned(r->q, 16) || unaligned(r->q_out, 16) || (r->ldq | r->ldqo) % 4))
+        return refuse(op, "q and q_out rows must be 16-byte aligned");
+    if (r->heads && (r->ldq < r->heads * hd || r->ldqo < r->heads * hd || (r->ldq | r->ldqo) > 0x7fffffffu))
+        return refuse(op, "ldq and ldqo must hold a row");
+    if (r->q_out && r->q_out == r->q && r->ldqo != r->ldq) return refuse(op, "rows turned in place keep their stride");
+    if (r->rot_dim % 8 || r->rot_dim > hd) return refuse(op, "rot_dim must be a multiple of 8 up to head_dim");
+    if (r->rot_dim && (unaligned(r->cos_t, 16) || unaligned(r->sin_t, 16) || r->max_pos < 1 || r->max_pos > 0x7fffffffu))
+        return refuse(op, "a rotation needs 16-byte aligned tables and max_pos");
+    if (!s->n || !s->rows) return 0;
+    KvAppendParams p;
+    memset(&p, 0, sizeof(p));
+    p.kv = paged_kv(c, s);
+    p.q = (const float*)r->q; p.k = (const float*)r->k; p.v = (const float*)r->v; p.q_out = (float*)r->q_out;
+    p.cos_t = (const float*)r->cos_t; p.sin_t = (const float*)r->sin_t;
+    p.ldq = (int)r->ldq; p.ldk = (int)r->ldk; p.ldv = (int)r->ldv; p.ldqo = (int)r->ldqo;
+    p.heads = (int)r->heads;
+    p.max_pos = (int)r->max_pos; p.rot = (int)r->rot_dim; p.rot_half = r->rot_half != 0;
+    const i32 i = hd_index(hd);
+    const u32 heads = r->heads + 2 * c->kv_heads;
+    const int four = four_rows(s->rows, hd, heads);
+    void* args[] = { &p };
+    hip_launch(kernel_hd(e, &e->append[i][c->type][four], four ? "k_kv_append4" : "k_kv_append", i, (i32)c->type),
+               (u32)cdiv64(s->rows, (four ? 4 : 1) * (1024 / hd)), heads, 1, 256, 1, 1, 0, args);
+    return 0;
+}
+
+i32 trlm_kv_read(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hipDeviceptr_t k_out, hipDeviceptr_t v_out,
+                 u32 ld) {
+    static const char* op = "trlm_kv_read";
+    const char* why = handle_fault(e);
+    if (!why) why = cache_fault(c, s);
+    if (why) return refuse(op, why);
+    const u32 hd = c->head_dim;
+    if (unaligned(k_out, 16) || unaligned(v_out, 16) || ld % 4) return refuse(op, "output rows must be 16-byte aligned");
+    if (ld < c->kv_heads * hd || ld > 0x7fffffffu) return refuse(op, "ld must hold a row");
+    if (!s->n || !s->rows) return 0;
+    KvReadParams p;
+    memset(&p, 0, sizeof(p));
+    p.kv = paged_kv(c, s);
+    p.k_out = (float*)k_out; p.v_out = (float*)v_out;
+    p.ld = (int)ld;
+    const i32 i = hd_index(hd);
+    const u32 heads = 2 * c->kv_heads;
+    const int four = four_rows(s->rows, hd, heads);
+    void* args[] = { &p };
+    hip_launch(kernel_hd(e, &e->read[i][c->type][four], four ? "k_kv_read4" : "k_kv_read", i, (i32)c->type),
+               (u32)cdiv64(s->rows, (four ? 4 : 1) * (1024 / hd)), heads, 1, 256, 1, 1, 0, args);
+    return 0;
+}
+
+/* ---------------- attention ---------------- */
+
+#define FEW_ROWS 16u      /* rows of a k_paged_attn_few workgroup */
+#define FEW_KEYS 128u     /* keys its four waves take at a time: splits are multiples of it */
+#define FEW_GROUPS 1024u  /* workgroups wanted: four for each of the 256 compute units */
+#define MAX_SPLITS 256u
+
+typedef struct AttnPlan { u32 tiles, splits, chunk; u64 groups; } AttnPlan;
+
+static u32 max_kv_of(const TrlmKvCache* c, const TrlmKvSeqs* s) {
+    const u64 held = (u64)s->max_pages * c->page_size;
+    return s->max_kv > held ? (u32)held : s->max_kv;
+}
+
+/* A call's launch shape, from what the host knows of it alone, so that a
+ * captured call keeps it. */
+static AttnPlan attn_plan(const TrlmKvCache* c, const TrlmKvSeqs* s, u32 heads) {
+    AttnPlan p;
+    const u32 group = heads / c->kv_heads, max_q = s->max_q < s->rows ? s->max_q : s->rows, kv = max_kv_of(c, s);
+    p.tiles = (u32)cdiv64((u64)max_q * group, FEW_ROWS);
+    p.groups = (u64)s->n * c->kv_heads * p.tiles;
+    u64 want = p.groups ? cdiv64(FEW_GROUPS, p.groups) : 1;
+    if (want > MAX_SPLITS) want = MAX_SPLITS;
+    p.chunk = (u32)(cdiv64(cdiv64(kv ? kv : 1, want), FEW_KEYS) * FEW_KEYS);
+    p.splits = (u32)cdiv64(kv ? kv : 1, p.chunk);
+    return p;
+}
+
+static u64 attn_ws(const TrlmKvCache* c, const TrlmKvSeqs* s, u32 heads, const AttnPlan* p) {
+    return p->splits > 1 ? (u64)s->rows * heads * p->splits * (c->head_dim + 2) * sizeof(f32) : 0;
+}
+
+u64 trlm_attn_paged_workspace(const TrlmKvCache* c, const TrlmKvSeqs* s, u32 heads) {
+    if (cache_fault(c, s) || !heads || heads > 1024 || heads % c->kv_heads || !s->n || !s->rows || !s->max_q) return 0;
+    const AttnPlan p = attn_plan(c, s, heads);
+    return attn_ws(c, s, heads, &p);
+}
+
+i32 trlm_attn_paged(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hipDeviceptr_t q, u32 ldq, u32 heads,
+                    f32 scale, hipDeviceptr_t out, u32 ldo, hipDeviceptr_t ws, u64 ws_bytes) {
+    static const char* op = "trlm_attn_paged";
+    const char* why = handle_fault(e);
+    if (!why) why = cache_fault(c, s);
+    if (why) return refuse(op, why);
+    const u32 hd = c->head_dim;
+    if (!heads || heads > 1024 || heads % c->kv_heads) return refuse(op, "heads must be a multiple of kv_heads, up to 1024");
+    if (unaligned(q, 16) || unaligned(out, 16) || (ldq | ldo) % 4) return refuse(op, "q and out rows must be 16-byte aligned");
+    if (ldq < heads * hd || ldo < heads * hd || (ldq | ldo) > 0x7fffffffu) return refuse(op, "ldq and ldo must hold a row");
+    if (!s->n || !s->rows || !s->max_q) return 0;
+    const AttnPlan pl = attn_plan(c, s, heads);
+    const u64 need = attn_ws(c, s, heads, &pl);
+    if (need && (unaligned(ws, 16) || ws_bytes < need)) return refuse(op, "the workspace is too small or not 16-byte aligned");
+    if (pl.groups > 0x7fffffffull || cdiv64((u64)s->rows * heads, 1024 / hd) > 0x7fffffffull)
+        return refuse(op, "too many workgroups");
+    PagedAttnParams p;
+    memset(&p, 0, sizeof(p));
+    p.kv = paged_kv(c, s);
+    p.q = (const float*)q; p.out = (float*)out;
+    p.part_o = (float*)ws;
+    p.part_ml = need ? (float*)ws + (u64)s->rows * heads * pl.splits * hd : NULL;
+    p.ldq = (int)ldq; p.ldo = (int)ldo; p.heads = (int)heads;
+    p.max_q = (int)(s->max_q < s->rows ? s->max_q : s->rows);
+    p.max_kv = (int)max_kv_of(c, s);
+    p.splits = (int)pl.splits; p.chunk = (int)pl.chunk;
+    p.scale = scale;
+    const i32 i = hd_index(hd);
+    void* args[] = { &p };
+    hip_launch(kernel_hd(e, &e->few[i][c->type], "k_paged_attn_few", i, (i32)c->type), (u32)pl.groups, pl.splits, 1, 256,
+               1, 1, 0, args);
+    if (pl.splits > 1)
+        hip_launch(kernel_hd(e, &e->join[i], "k_paged_attn_join", i, -1),
+                   (u32)cdiv64((u64)s->rows * heads, 1024 / hd), 1, 1, 256, 1, 1, 0, args);
+    return 0;
+}
+
+/* ---------------- rules on logits ---------------- */
+
+/* Tokens a workgroup takes of its row: 4096, or 1024 where that leaves fewer
+ * than two workgroups for each of the 256 compute units. */
+#define RULES_WIDE 4096u
+#define RULES_NARROW 1024u
+
+i32 trlm_logits_rules(TrlmServe* e, const TrlmLogitsRules* r) {
+    static const char* op = "trlm_logits_rules";
+    const char* why = handle_fault(e);
+    if (why) return refuse(op, why);
+    if (!r) return refuse(op, "no rules");
+    if (unaligned(r->logits, 4) || unaligned(r->out, 4)) return refuse(op, "logits and out must be device buffers");
+    if (r->vocab < 1 || r->vocab > (1u << 30) || r->ld < r->vocab || r->ld_out < r->vocab)
+        return refuse(op, "vocab must be 1 to 2^30 and ld, ld_out at least vocab");
+    if (r->rows > 65535) return refuse(op, "more than 65535 rows");
+    if (r->out == r->logits && r->ld != r->ld_out) return refuse(op, "rules in place keep the rows' stride");
+    if (r->history && (unaligned(r->history, 4) || unaligned(r->hist_len, 4) || !r->ld_hist || r->ld_hist > (1u << 30)))
+        return refuse(op, "a history needs its lengths and ld_hist, 1 to 2^30");
+    if (r->bias_ids && (unaligned(r->bias_ids, 4) || unaligned(r->bias, 4) || unaligned(r->n_bias, 4) || !r->ld_bias ||
+                        r->ld_bias > (1u << 30)))
+        return refuse(op, "biases need their ids, values, counts and ld_bias, 1 to 2^30");
+    if (r->mask && (unaligned(r->mask, 4) || r->ld_mask < (r->vocab + 31) / 32))
+        return refuse(op, "ld_mask must be at least ceil(vocab / 32)");
+    if (!r->rows) return 0;
+    RulesParams p;
+    memset(&p, 0, sizeof(p));
+    p.logits = (const float*)r->logits; p.out = (float*)r->out;
+    p.history = (const unsigned*)r->history; p.hist_len = (const int*)r->hist_len; p.gen_start = (const int*)r->gen_start;
+    p.repetition = (const float*)r->repetition; p.frequency = (const float*)r->frequency;
+    p.presence = (const float*)r->presence;
+    p.bias_ids = (const unsigned*)r->bias_ids; p.bias = (const float*)r->bias; p.n_bias = (const int*)r->n_bias;
+    p.mask = (const unsigned*)r->mask;
+    p.ld = r->ld; p.ld_out = r->ld_out; p.ld_hist = r->ld_hist; p.ld_bias = r->ld_bias; p.ld_mask = r->ld_mask;
+    p.vocab = (int)r->vocab;
+    const int u = unaligned(r->logits, 16) || unaligned(r->out, 16) || (r->ld | r->ld_out) % 4;
+    const int wide = cdiv64(r->vocab, RULES_WIDE) * r->rows >= 512;
+    static const char* const NAMES[2][2] = { { "k_logits_rules_1024", "k_logits_rules_1024_u" },
+                                             { "k_logits_rules_4096", "k_logits_rules_4096_u" } };
+    void* args[] = { &p };
+    hip_launch(kernel(e, &e->rules[wide][u], NAMES[wide][u]), (u32)cdiv64(r->vocab, wide ? RULES_WIDE : RULES_NARROW),
+               r->rows, 1, 256, 1, 1, 0, args);
+    return 0;
+}

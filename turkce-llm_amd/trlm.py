@@ -95,6 +95,41 @@ class TrlmSchedule(C.Structure):
                 ("seed_base", C.c_uint64)]
 
 
+# How a paged cache holds its numbers (trlm_serve.h)
+KV_F32, KV_BF16, KV_I8 = 0, 1, 2
+
+
+class KvCache(C.Structure):
+    """Mirror of TrlmKvCache (trlm_serve.h): one layer's pool of pages."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("type", C.c_uint32), ("num_pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class KvSeqs(C.Structure):
+    """Mirror of TrlmKvSeqs: the sequences of a call."""
+    _fields_ = [("n", C.c_uint32), ("rows", C.c_uint32), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("pages", C.c_void_p), ("max_pages", C.c_uint32), ("max_q", C.c_uint32), ("max_kv", C.c_uint32)]
+
+
+class KvRows(C.Structure):
+    """Mirror of TrlmKvRows: the new tokens' rows and their rotation."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("ldq", C.c_uint32), ("ldk", C.c_uint32),
+                ("ldv", C.c_uint32), ("q_out", C.c_void_p), ("ldqo", C.c_uint32), ("heads", C.c_uint32),
+                ("cos_t", C.c_void_p), ("sin_t", C.c_void_p), ("max_pos", C.c_uint32), ("rot_dim", C.c_uint32),
+                ("rot_half", C.c_uint32)]
+
+
+class LogitsRules(C.Structure):
+    """Mirror of TrlmLogitsRules: penalties, biases and masks of rows of logits."""
+    _fields_ = [("logits", C.c_void_p), ("out", C.c_void_p), ("rows", C.c_uint32), ("vocab", C.c_uint32),
+                ("ld", C.c_uint32), ("ld_out", C.c_uint32), ("history", C.c_void_p), ("hist_len", C.c_void_p),
+                ("gen_start", C.c_void_p), ("ld_hist", C.c_uint32), ("repetition", C.c_void_p),
+                ("frequency", C.c_void_p), ("presence", C.c_void_p), ("bias_ids", C.c_void_p),
+                ("bias", C.c_void_p), ("n_bias", C.c_void_p), ("ld_bias", C.c_uint32), ("mask", C.c_void_p),
+                ("ld_mask", C.c_uint32)]
+
+
 _libs = None
 
 
@@ -240,6 +275,15 @@ def _bind(host, hip):
     _sig(hip, "node_matmul2d_gpu", NodeP, [AP, NodeP, NodeP])
     _sig(hip, "gpu_ops_debug_stats", None, [C.POINTER(C.c_double), C.POINTER(C.c_uint32)])
     _sig(hip, "gpu_ops_debug_reset", None, [])
+    cache, seqs = C.POINTER(KvCache), C.POINTER(KvSeqs)
+    _sig(hip, "trlm_serve_create", C.c_void_p, [HP])
+    _sig(hip, "trlm_serve_destroy", None, [C.c_void_p])
+    _sig(hip, "trlm_kv_append", C.c_int32, [C.c_void_p, cache, seqs, C.POINTER(KvRows)])
+    _sig(hip, "trlm_kv_read", C.c_int32, [C.c_void_p, cache, seqs, C.c_void_p, C.c_void_p, C.c_uint32])
+    _sig(hip, "trlm_attn_paged_workspace", C.c_uint64, [cache, seqs, C.c_uint32])
+    _sig(hip, "trlm_attn_paged", C.c_int32, [C.c_void_p, cache, seqs, C.c_void_p, C.c_uint32, C.c_uint32, C.c_float,
+                                             C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint64])
+    _sig(hip, "trlm_logits_rules", C.c_int32, [C.c_void_p, C.POINTER(LogitsRules)])
     _sig(hip, "gpu_ops_pin", None, [C.c_void_p, C.c_uint64])
     _sig(hip, "gpu_ops_unpin_all", None, [])
 
@@ -598,3 +642,41 @@ class Device:
         self.current()   # the engine's workspace is freed in its own context
         self.hip.trlm_gemm_destroy(self.gemm)
         self.hip.hip_shutdown(C.byref(self.ctx))
+
+
+class Refused(ValueError):
+    """A serving operator refused its arguments (the reason is on stderr)."""
+
+
+class Serve:
+    """The serving operators (trlm_serve.h) in a Device's context, queued on
+    its stream: device pointers in, nothing waited for."""
+
+    def __init__(self, dev):
+        self.hip = dev.hip
+        self.e = self.hip.trlm_serve_create(C.byref(dev.ctx))
+
+    @staticmethod
+    def _checked(rc, what):
+        if rc != 0:
+            raise Refused(what)
+
+    def append(self, cache, seqs, rows):
+        self._checked(self.hip.trlm_kv_append(self.e, cache, seqs, rows), "trlm_kv_append")
+
+    def read(self, cache, seqs, k_out, v_out, ld):
+        self._checked(self.hip.trlm_kv_read(self.e, cache, seqs, k_out, v_out, ld), "trlm_kv_read")
+
+    def attn_workspace(self, cache, seqs, heads):
+        return self.hip.trlm_attn_paged_workspace(cache, seqs, heads)
+
+    def attn(self, cache, seqs, q, ldq, heads, scale, out, ldo, ws=None, ws_bytes=0):
+        self._checked(self.hip.trlm_attn_paged(self.e, cache, seqs, q, ldq, heads, scale, out, ldo, ws, ws_bytes),
+                      "trlm_attn_paged")
+
+    def logits_rules(self, rules):
+        self._checked(self.hip.trlm_logits_rules(self.e, rules), "trlm_logits_rules")
+
+    def close(self):
+        self.hip.trlm_serve_destroy(self.e)
+        self.e = None

@@ -116,10 +116,13 @@ def rotate(x, cos, sin, rot, half):
 
 def attention(pool, seqs, q, H, scale):
     """(out, bound) in 64 bits: out [rows, H, hd] (zeros where nothing is seen) and for each row and head how far fp32
-    arithmetic may be off.  With u = 2^-24 and A the largest scale log2(e) sum |q_d k_d| of the keys seen: a score is
-    off by at most (hd + 8) u A (hd products and sums, the query's scaling, the splits), a weight relatively by ln 2
-    times that of it and of the maximum, and 2^-22 for the power; a sum of n weights by n u; numerator and denominator
-    both: max|v| (4 ln2 A (hd + 8) u + 2 n u + 2^-21)."""
+    arithmetic may be off.  With u = 2^-24, a score in units of log2 is off by at most (hd + 8) u A_t, A_t = scale
+    log2(e) sum |q_d k_d| (hd products and sums, the query's scaling, the operands' 22 to 24 bits), and by 2^-29 of the
+    row's largest number times the other operand's magnitudes (what the operands' splits leave): a weight relatively by
+    d_t = ln 2 times that, 2^-22 for the power and its split, and n u for the sum over n weights.  What all weights
+    share cancels.  Numerator and denominator: (sum w_t |v_t| d_t + sum w_t d_t sum w_t |v_t| / sum w_t) / sum w_t, |v_t|
+    the row's largest; twice, for the splits and their join, and
+    2^-120 where values come near the end of fp32's range."""
     hd, G = pool.hd, H // pool.Hkv
     out = np.zeros((seqs.rows, H, hd))
     bound = np.zeros((seqs.rows, H))
@@ -137,8 +140,10 @@ def attention(pool, seqs, q, H, scale):
                 z = k @ x * scale
                 w = np.exp(z - z.max())
                 out[r0 + j, h] = w @ v / w.sum()
-                A = np.abs(scale) * 1.4427 * (np.abs(k) @ np.abs(x)).max()
-                bound[r0 + j, h] = np.abs(v).max() * (4 * 0.6932 * A * (hd + 8) * u + 2 * see.size * u + 2.0 ** -21)
+                ak, ax, top = np.abs(k), np.abs(x), np.abs(v).max(1)
+                A = ak @ ax * (hd + 8) * u + (ak.max(1) * ax.sum() + ak.sum(1) * ax.max()) * 2.0 ** -29
+                d = 0.6932 * np.abs(scale) * 1.4427 * A + 2.0 ** -22 + see.size * u
+                bound[r0 + j, h] = 2 * (w @ (top * d) + (w @ d) * (w @ top) / w.sum()) / w.sum() + 2.0 ** -120
     return out, bound
 
 

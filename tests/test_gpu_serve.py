@@ -205,7 +205,7 @@ def test_append_rows_at_the_ends_of_the_range(trlm, box):
 # ---------------------------------------------------------------- attention
 
 def attn_case(trlm, box, rng, type, hd, H, Hkv, q_len, kv_len, page, spare_rows=0, pad=0, garbage=None, tables_of=None,
-              max_q=None, max_kv=None, scale=None, std=1.0):
+              max_q=None, max_kv=None, scale=None, std=1.0, numbers=None):
     """trlm_attn_paged against serve_ref.attention; returns (out, want, seqs)."""
     dev, serve = box
     dev.current()
@@ -217,8 +217,10 @@ def attn_case(trlm, box, rng, type, hd, H, Hkv, q_len, kv_len, page, spare_rows=
     if max_kv:
         seqs.max_kv = max_kv
     shape = (seqs.num, Hkv, page, hd)
-    pool = ref.Pool(type, seqs.num, page, Hkv, hd, std * rng.standard_normal(shape).astype(np.float32),
-                    rng.standard_normal(shape).astype(np.float32))
+    kv = [std * rng.standard_normal(shape).astype(np.float32), rng.standard_normal(shape).astype(np.float32)]
+    if numbers is not None:
+        numbers(rng, *kv)
+    pool = ref.Pool(type, seqs.num, page, Hkv, hd, *kv)
     ldq, ldo = H * hd + pad, H * hd + 2 * pad
     q = std * rng.standard_normal((seqs.rows, ldq)).astype(np.float32)
     scale = 1.0 / math.sqrt(hd) if scale is None else scale
@@ -380,6 +382,44 @@ def test_attn_flat_and_sharp(trlm, box, std):
     """Nearly equal weights and nearly one-hot ones."""
     rng = np.random.default_rng(31)
     attn_case(trlm, box, rng, "f32", 64, 2, 2, [1, 70], [300, 300], 32, std=std)
+
+
+def rows_of_all_sizes(rng, k, v):
+    """Key and value rows of magnitudes 2^-30 .. 2^30 in no order (keys: to 2^6), some of zeros alone."""
+    shape = k.shape[:3] + (1,)
+    k *= (2.0 ** rng.integers(-30, 7, shape)).astype(np.float32)
+    v *= (2.0 ** rng.integers(-30, 31, shape)).astype(np.float32)
+    k[rng.random(k.shape[:3]) < 0.1] = 0
+    v[rng.random(k.shape[:3]) < 0.1] = 0
+
+
+def pages_of_all_sizes(rng, k, v):
+    """Magnitudes that change from page to page, to the ends of fp32's range for values."""
+    k *= (2.0 ** rng.integers(-20, 5, (k.shape[0], 1, 1, 1))).astype(np.float32)
+    v *= (2.0 ** rng.integers(-120, 121, (k.shape[0], 1, 1, 1))).astype(np.float32)
+
+
+def weightless_giants(rng, k, v):
+    """Every eighth key against the queries' mean with a value 2^60 times the others': its weight is 0."""
+    k[:, :, ::8] = 0
+    k[:, :, ::8, 0] = -3000
+    v[:, :, ::8] *= np.float32(2.0 ** 60)
+
+
+@pytest.mark.parametrize("numbers", [rows_of_all_sizes, pages_of_all_sizes, weightless_giants])
+@pytest.mark.parametrize("type", ALL_TYPES)
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_attn_numbers_of_every_magnitude(trlm, box, numbers, type, hd):
+    """Neighbours of very different size do not cost one another's precision; single tokens and chunks."""
+    rng = np.random.default_rng(47)
+    attn_case(trlm, box, rng, type, hd, 2, 1, [1, 70, 2, 150], [77, 130, 200, 150], 16, numbers=numbers)
+
+
+@pytest.mark.parametrize("std", [2.0 ** -40, 2.0 ** 20])
+def test_attn_queries_of_every_magnitude(trlm, box, std):
+    """A chunk whose queries are scaled row by row; the scale argument undoes the mean of it."""
+    rng = np.random.default_rng(53)
+    attn_case(trlm, box, rng, "f32", 64, 2, 2, [1, 100], [100, 300], 32, std=std, scale=0.125 / std / std)
 
 
 def test_attn_repeats_bit_for_bit(trlm, box):

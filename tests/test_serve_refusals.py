@@ -263,7 +263,8 @@ def test_header_and_binding_agree(trlm, tmp_path):
 
 
 def kernel_names():
-    names = {"k_%s_hd%d_%s" % (k, hd, t) for k in ("kv_append", "kv_append4", "kv_read", "kv_read4", "paged_attn_few")
+    names = {"k_%s_hd%d_%s" % (k, hd, t) for k in ("kv_append", "kv_append4", "kv_read", "kv_read4", "paged_attn_few", "paged_attn_tile4",
+                                                  "paged_attn_tile8")
              for hd in (16, 32, 64, 128) for t in ("f32", "bf16", "i8")}
     names |= {"k_paged_attn_join_hd%d" % hd for hd in (16, 32, 64, 128)}
     return names | {"k_logits_rules_%d%s" % (w, u) for w in (1024, 4096) for u in ("", "_u")}

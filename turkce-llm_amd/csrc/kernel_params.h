@@ -134,7 +134,9 @@ typedef struct PagedAttnParams {
     float* part_ml;          // [row][head][splits][2]: its base-2 maximum and its sum of weights
     int ldq, ldo, heads;
     int max_q, max_kv;
-    int splits, chunk;       // keys [s * chunk, (s + 1) * chunk) of a sequence are split s
+    int few_rows;            // sequences of at most so many rows (tokens x group) go to the few-rows kernel
+    int splits;              // slots of a row's parts
+    int chunk_few, chunk_tile;   // keys [s * chunk, (s + 1) * chunk) of a sequence are split s
     float scale;
 } PagedAttnParams;
 

@@ -123,7 +123,8 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, kq = lane >> 4;
     const int G = p.heads / c.kv_heads;
-    const int tiles = (p.max_q * G + 15) >> 4;
+    const int most = p.max_q * G < p.few_rows ? p.max_q * G : p.few_rows;
+    const int tiles = (most + 15) >> 4;
     int x = blockIdx.x;
     const int tile = x % tiles;
     x /= tiles;
@@ -134,7 +135,7 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
     q1 = q1 > c.rows ? c.rows : q1;
     const int qn = q1 - q0 < p.max_q ? q1 - q0 : p.max_q;
     const int R = qn * G, r0 = tile * 16;
-    if (r0 >= R) return;
+    if (r0 >= R || R > p.few_rows) return;
     const int held = c.kv_len[seq];
     const int keys = held < 0 ? 0 : held > p.max_kv ? p.max_kv : held;
     const int nr = R - r0 < 16 ? R - r0 : 16;
@@ -148,9 +149,9 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
     const int lim = limit(tok);
     const int lim_hi = limit((r0 + nr - 1) / G), lim_lo = limit(r0 / G);
     const int split = blockIdx.y;
-    const int c0 = split * p.chunk;
+    const int c0 = split * p.chunk_few;
     if (split > 0 && c0 >= lim_hi) return;
-    const int c1 = c0 + p.chunk < lim_hi ? c0 + p.chunk : lim_hi;
+    const int c1 = c0 + p.chunk_few < lim_hi ? c0 + p.chunk_few : lim_hi;
     for (int d = threadIdx.x; d < HD; d += 256) bad[d] = PA_NONE;
     __syncthreads();
 
@@ -303,7 +304,7 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
 #pragma unroll
         for (int e = 0; e < VD; e++) wo[wave][i][(4 * kq + r) * VD + e] = o[e][r];
     __syncthreads();
-    const bool last = keys <= p.chunk;        // the sequence has one split: no other part to join
+    const bool last = keys <= p.chunk_few;        // the sequence has one split: no other part to join
     for (int at = threadIdx.x; at < nr * (HD / 4); at += 256) {
         const int r = at / (HD / 4), d = 4 * (at % (HD / 4));
         const int t = (r0 + r) / G, head = h * G + (r0 + r) - t * G;
@@ -336,6 +337,532 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
     }
 }
 
+// ------------------------------------------------------------------ many rows
+// A workgroup takes 32 NW rows of one cached head over one split of its keys;
+// every wave has 32 rows and all the keys, which pass through LDS in tiles of
+// KB, double-buffered: while a tile is computed, the next is in LDS or on its
+// way there and the one after it in flight from memory, one barrier a tile.
+//
+// Products on the f16 matrix cores (v_mfma_f32_32x32x16_f16): fp32 numbers as
+// two f16 terms (22 bits and the sign of the second), products of three of
+// their four partial products (the fourth is below 2^-22 of it, as fp32's own
+// rounding is); bf16 and 8-bit numbers are one f16 number, two partial
+// products.  Against three bf16 terms this halves the products for fp32 caches
+// and saves a third for the others, and splitting a weight costs 1.5 VALU
+// instructions for 5.5.  f16's range is met by powers of two that change
+// nothing else:
+//   a row of Q is scaled by its own largest magnitude;
+//   keys are scaled by one power for a tile, values by another, which puts
+//     their rows' largest magnitudes into [2^5, 2^15) (two terms are good to
+//     22 bits of a number and to 2^-25: 30 bits of its row's largest at least);
+//   with V' = 2^-ev V a second running maximum mo is kept, of s + ev: weights
+//     2^(s + ev - mo + 14) <= 2^14 are small against the largest contribution to
+//     the row, not against the largest weight; their sum is taken back to m.
+// The powers of a tile are those of the tile before it.  A tile whose rows do
+// not fit them (the first one, or rows of very different magnitude next to one
+// another) is taken again by classes of keys that fit one pair of powers,
+// largest first, the others masked; the last pair stays.  Numbers that are not
+// finite leave the products: the first such key of each column of V, and of
+// K, is kept, and rows that see it get NaN at the end.
+//
+// S^T = K Q^T puts a row into a lane's column, as in attention.hip, and the
+// exponentiated result is operand B of O^T += V^T P^T as it is: registers 8 u
+// .. 8 u + 7 of lane half h are the keys 16 u + 8 a + 4 h + c (a < 2, c < 4).
+// V^T is read from V's own rows by ds_read_b64_tr_b16: of 16 lanes, lanes 4 e ..
+// 4 e + 3 address 16 numbers of row e, and lane j receives number j of rows 0 .. 3.
+typedef _Float16 pa_f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 pa_f16x8 __attribute__((ext_vector_type(8)));
+typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) pa_s16x4 pa_lds_s16x4;
+
+#define PA_EXP_MIN 12      // rows below 2^-115 take the power of 2^-115 (their scale is then 2^126)
+#define PA_W 14            // a row's weights go up to 2^14
+#define PA_UP 11           // a row's largest magnitude goes to about 2^11 ..
+#define PA_ABOVE 3         // .. and may be up to 2^3 above that
+#define PA_BELOW 6         // .. or 2^6 below
+#define PA_I8_UP 4         // 8-bit integers: times 2^4
+
+__device__ __forceinline__ float pa_pow2(int e) {       // 2^e, e kept in [-126, 127]
+    e = e < -126 ? -126 : e > 127 ? 127 : e;
+    return __uint_as_float((unsigned)(e + 127) << 23);
+}
+
+// Maximum over the N lanes (a power of two up to 16) that share a row.
+template <int N>
+__device__ __forceinline__ unsigned pa_row_max(unsigned v) {
+    if (N >= 2) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));    // lane ^ 1
+    if (N >= 4) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));    // lane ^ 2
+    if (N >= 8) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));   // 7 - lane of 8
+    if (N >= 16) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, false));  // 15 - lane of 16
+    return v;
+}
+
+__device__ __forceinline__ int pa_wave_max(int v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = max(v, __shfl_xor(v, o, WAVE));
+    return v;
+}
+
+template <int HD, int TYPE, int NW, int KB>
+__device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
+    constexpr int THREADS = 64 * NW, NT = TYPE == KV_F32 ? 2 : 1;
+    constexpr int CPR = HD / 8, CH = KB * CPR, CK = (CH + THREADS - 1) / THREADS;   // 8-number chunks
+    constexpr int NS = HD / 16, DB = (HD + 31) / 32, KT = KB / 32;
+    static_assert(KB <= 64 && CH % 64 == 0 && (CH % THREADS == 0 || CH < THREADS), "chunks of whole waves");
+    __shared__ __attribute__((aligned(16))) pa_u32x4 kbuf[2][NT][CH], vbuf[2][NT][CH];
+    __shared__ __attribute__((aligned(16))) float ksc[TYPE == KV_I8 ? 2 : 1][KB], vsc[TYPE == KV_I8 ? 2 : 1][KB];
+    __shared__ int misfit[2], kbad, bad[HD], lek[KB], lev[KB];
+    const PagedKv& c = p.kv;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int G = p.heads / c.kv_heads;
+    const int tiles = (p.max_q * G + 32 * NW - 1) / (32 * NW);
+    // the last rows (which see the most keys) first
+    int x = blockIdx.x;
+    const int h = x % c.kv_heads;
+    x /= c.kv_heads;
+    const int seq = x % c.n, tile = tiles - 1 - x / c.n;
+    int q0 = c.q_start[seq], q1 = c.q_start[seq + 1];
+    const int q1_said = q1;
+    q0 = q0 < 0 ? 0 : q0;
+    q1 = q1 > c.rows ? c.rows : q1;
+    const int qn = q1 - q0 < p.max_q ? q1 - q0 : p.max_q;
+    const int R = qn * G, r0 = tile * 32 * NW;
+    if (r0 >= R || R <= p.few_rows) return;
+    const int held = c.kv_len[seq];
+    const int keys = held < 0 ? 0 : held > p.max_kv ? p.max_kv : held;
+    const int nr = R - r0 < 32 * NW ? R - r0 : 32 * NW;
+    const int pos0 = held - (q1_said - q0);
+    auto limit = [&](int t) {
+        const int l = pos0 + t + 1;
+        return l < 0 ? 0 : l > keys ? keys : l;
+    };
+    const int lim_hi = limit((r0 + nr - 1) / G);
+    const int split = blockIdx.y, c0 = split * p.chunk_tile;
+    if (split > 0 && c0 >= lim_hi) return;
+    const int c1 = c0 + p.chunk_tile < lim_hi ? c0 + p.chunk_tile : lim_hi;
+    // this lane's row, and the keys that the wave's rows see
+    const int w0 = r0 + 32 * wave, w1 = (w0 + 31 < R ? w0 + 31 : R - 1);
+    const int row = w0 + (lane & 31) < R ? w0 + (lane & 31) : R - 1;
+    const int tok = row / G, head = h * G + row - tok * G;
+    const int lim = limit(tok);
+    const bool busy = w0 < R;
+    const int wave_lo = busy ? limit(w0 / G) : 0, wave_hi = busy ? limit(w1 / G) : 0;
+
+    if (threadIdx.x < 2) misfit[threadIdx.x] = -1;
+    if (threadIdx.x == 2) kbad = PA_NONE;
+    for (int d = threadIdx.x; d < HD; d += THREADS) bad[d] = PA_NONE;
+
+    // operand B of S^T: the row's numbers times scale log2(e), two f16 terms
+    pa_f16x8 qh[NS], ql[NS];
+    int qe;                                  // the row's numbers are its f16 numbers times 2^qe
+    bool qpoor;
+    {
+        const float* qr = p.q + (long long)(q0 + tok) * p.ldq + head * HD + 8 * half;
+        const float f = p.scale * PA_LOG2E;
+        f32x4 v[NS][2];
+        unsigned m = 0;
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                v[s][j] = *(const f32x4*)(qr + 16 * s + 4 * j) * f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) m = max(m, __float_as_uint(v[s][j][e]) & 0x7fffffffu);
+            }
+        m = max(m, (unsigned)__shfl_xor((int)m, 32, WAVE));
+        qpoor = m >= 0x7f800000u;
+        int e = (int)(m >> 23);
+        e = e < 20 ? 20 : e;
+        qe = e - 127 - PA_UP;
+        const float up = qpoor ? 0.f : pa_pow2(-qe);
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = qpoor ? 0.f : v[s][j / 4][j % 4] * up;
+                const _Float16 hi = (_Float16)y;
+                qh[s][j] = hi;
+                ql[s][j] = (_Float16)(y - (float)hi);
+            }
+    }
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.f;
+    float m = -INFINITY, l = 0.f, mo = -INFINITY;   // maxima of s (l's reference) and of s + ev (o's)
+
+    // ---- tiles: chunk i of a thread is numbers 8 cc .. + 7 of key ckey(i)
+    const int* table = c.pages + (long long)seq * c.max_pages;
+    const int cc = threadIdx.x % CPR;
+    auto ckey = [&](int i) { return (int)(threadIdx.x + i * THREADS) / CPR; };
+    const bool stages = CH >= THREADS || threadIdx.x < CH;
+    auto page_of = [&](int key) {
+        const int at = key >> c.page_shift;
+        return table[at < c.max_pages ? at : c.max_pages - 1];
+    };
+    // the pool row of a key, or -1 where it is not held or not seen
+    auto place_of = [&](int key, int page) -> long long {
+        if (key >= c1 || page < 0 || page >= c.num_pages) return -1;
+        return (((long long)page * c.kv_heads + h) << c.page_shift) + (key & ((1 << c.page_shift) - 1));
+    };
+    struct Raw {
+        PaRun<TYPE, 8> k, v;
+        float ks, vs;
+        bool in;
+    };
+    auto load = [&](Raw& r, long long place) {
+        r.in = place >= 0;
+        const long long at = r.in ? place : 0;
+        r.k.load(c.k, at * HD + 8 * cc);
+        r.v.load(c.v, at * HD + 8 * cc);
+        if (TYPE == KV_I8) {
+            r.ks = c.ks[at];
+            r.vs = c.vs[at];
+        }
+    };
+    int EK = 128, EV = TYPE == KV_I8 ? 124 : 128;   // powers for rows with numbers up to 4 (scales up to 2^-2)
+    // the eight numbers, their row's largest magnitude's bits; what is not
+    // finite becomes 0 and is noted (V: by column, K: by key)
+    auto numbers = [&](const PaRun<TYPE, 8>& run, bool in, bool is_k, int key, float (&y)[8]) -> unsigned {
+        unsigned big = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            y[e] = in ? run.get(e) : 0.f;
+            if (TYPE != KV_I8) big = max(big, __float_as_uint(y[e]) & 0x7fffffffu);
+        }
+        if (TYPE != KV_I8) {
+            if (big >= 0x7f800000u) {
+                big = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    if ((__float_as_uint(y[e]) & 0x7fffffffu) >= 0x7f800000u) {
+                        if (is_k) atomicMin(&kbad, key);
+                        else atomicMin(&bad[8 * cc + e], key);
+                        y[e] = 0.f;
+                    }
+                    big = max(big, __float_as_uint(y[e]) & 0x7fffffffu);
+                }
+            }
+            big = pa_row_max<CPR>(big);
+        }
+        return big;
+    };
+    // a row of zeros in K fits any power; in V it has the least one, so that a
+    // large weight on it does not stand before the others' contributions
+    auto exponent = [](unsigned big) { return max((int)(big >> 23), PA_EXP_MIN); };
+    // 8-bit scales: what is not finite as above
+    auto scale_of = [&](float s, bool in, bool is_k, int key) -> float {
+        if (!in) return 0.f;
+        if ((__float_as_uint(s) & 0x7fffffffu) >= 0x7f800000u) {
+            if (is_k) atomicMin(&kbad, key);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; e++) atomicMin(&bad[8 * cc + e], key);
+            return 0.f;
+        }
+        return s;
+    };
+    // one chunk into LDS under the current powers; whether its rows fit them
+    auto stage = [&](const Raw& r, bool in, int buf, int kk, int key) -> bool {
+        float y[8], z[8];
+        const unsigned bk = numbers(r.k, in, true, key, y);
+        const unsigned bv = numbers(r.v, in, false, key, z);
+        bool fits = true;
+        float uk, uv;
+        if (TYPE == KV_I8) {
+            const float s = scale_of(r.ks, in, true, key), t = scale_of(r.vs, in, false, key);
+            const int e = exponent(__float_as_uint(t) & 0x7fffffffu);
+            fits = !in || (e <= EV && e >= EV - PA_BELOW);
+            if (cc == 0) {
+                ksc[buf][kk] = s;
+                vsc[buf][kk] = t * pa_pow2(127 - EV);
+            }
+            uk = uv = (float)(1 << PA_I8_UP);
+        } else {
+            const int a = exponent(bk), b = exponent(bv);
+            fits = (bk == 0 || (a <= EK + PA_ABOVE && a >= EK - PA_BELOW)) &&
+                   (!in || (b <= EV + PA_ABOVE && b >= EV - PA_BELOW));
+            uk = pa_pow2(PA_UP + 127 - EK);
+            uv = pa_pow2(PA_UP + 127 - EV);
+        }
+        const int swk = CPR >= 8 ? (kk & 7) : CPR == 4 ? ((kk >> 1) & 3) : ((kk >> 2) & 1);
+        const int swv = CPR >= 8 ? (kk & 1) << 2 : 0;
+        pa_f16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float w = y[e] * uk;
+            hi[e] = (_Float16)w;
+            lo[e] = (_Float16)(w - (float)hi[e]);
+        }
+        kbuf[buf][0][kk * CPR + (cc ^ swk)] = __builtin_bit_cast(pa_u32x4, hi);
+        if (NT == 2) kbuf[buf][NT - 1][kk * CPR + (cc ^ swk)] = __builtin_bit_cast(pa_u32x4, lo);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float w = z[e] * uv;
+            hi[e] = (_Float16)w;
+            lo[e] = (_Float16)(w - (float)hi[e]);
+        }
+        vbuf[buf][0][kk * CPR + (cc ^ swv)] = __builtin_bit_cast(pa_u32x4, hi);
+        if (NT == 2) vbuf[buf][NT - 1][kk * CPR + (cc ^ swv)] = __builtin_bit_cast(pa_u32x4, lo);
+        return fits;
+    };
+    // the keys of a tile that have a place and are seen by some row
+    auto live_keys = [&](int b) -> unsigned long long {
+        unsigned long long live = 0;
+#pragma unroll
+        for (int g = 0; g < KB / 16; g++) {
+            const int page = page_of(b + 16 * g);
+            if (page >= 0 && page < c.num_pages) live |= 0xffffull << (16 * g);
+        }
+        const int left = c1 - b;
+        return left >= 64 ? live : live & ((1ull << (left > 0 ? left : 0)) - 1);
+    };
+
+    // ---- one tile of LDS into this wave's rows
+    auto compute = [&](int buf, int b, unsigned long long live) {
+        constexpr unsigned long long ALL = KB == 64 ? ~0ull : (1ull << (KB & 63)) - 1;
+        f32x16 s[KT];
+        const int r = lane & 31;
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[t][e] = 0.f;
+            const int kk = 32 * t + r;
+            const int sw = CPR >= 8 ? (kk & 7) : CPR == 4 ? ((kk >> 1) & 3) : ((kk >> 2) & 1);
+#pragma unroll
+            for (int n = 0; n < NS; n++) {
+                const pa_f16x8 kh = __builtin_bit_cast(pa_f16x8, kbuf[buf][0][kk * CPR + ((2 * n + half) ^ sw)]);
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[n], s[t], 0, 0, 0);
+                if (NT == 2) {
+                    const pa_f16x8 kl = __builtin_bit_cast(pa_f16x8, kbuf[buf][NT - 1][kk * CPR + ((2 * n + half) ^ sw)]);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[n], s[t], 0, 0, 0);
+                }
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[n], s[t], 0, 0, 0);
+            }
+            if (TYPE == KV_I8) {
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const f32x4 f = *(const f32x4*)&ksc[buf][32 * t + 8 * g + 4 * half];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[t][4 * g + e] *= f[e];
+                }
+            }
+        }
+        if (live != ALL || b + KB > wave_lo) {
+            const int seen = lim - b - 4 * half;
+#pragma unroll
+            for (int t = 0; t < KT; t++) {
+                const unsigned lt = (unsigned)(live >> (32 * t)) >> (4 * half);
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int kk = 8 * (e >> 2) + (e & 3);
+                    if (32 * t + kk >= seen || !(lt >> kk & 1)) s[t][e] = -INFINITY;
+                }
+            }
+        }
+        const float cu = pa_pow2(qe + (TYPE == KV_I8 ? -PA_I8_UP : EK - 127 - PA_UP));
+        const float ev = (float)(EV - 127 - (TYPE == KV_I8 ? PA_I8_UP : PA_UP));
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(s[t][e], s[t][e + 1]));
+        top = fmaxf(top, __shfl_xor(top, 32, WAVE)) * cu;
+        // (a row that has seen no key yet: references of 0, and zeros)
+        const float mo_new = fmaxf(mo, top + ev), m_new = fmaxf(m, top);
+        const float ref = m_new == -INFINITY ? 0.f : m_new, refo = m_new == -INFINITY ? 0.f : mo_new;
+        const float alpha = __builtin_amdgcn_exp2f(mo - refo);
+        l *= __builtin_amdgcn_exp2f(m - ref);
+        m = m_new;
+        mo = mo_new;
+        // a weight 2^(s - ref) is 2^gap of the same key's 2^(s + ev - refo + W)
+        const float off = (float)PA_W + ev - refo, gap = -off - ref;
+        const bool far = __ballot(gap > 60.0f) != 0;
+        float sum = 0.f;
+        if (far) {
+            // values so much smaller than another key's that their weights
+            // would leave fp32's range beside it: summed on their own
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], cu, -ref));
+            l += sum;
+        }
+        sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], cu, off));
+                sum += w;
+                s[t][e] = w;
+            }
+            if (TYPE == KV_I8) {
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const f32x4 f = *(const f32x4*)&vsc[buf][32 * t + 8 * g + 4 * half];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[t][4 * g + e] *= f[e];
+                }
+            }
+        }
+        if (!far) l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(gap), l);
+        if (__ballot(alpha != 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= alpha;
+        }
+        const int i = lane & 15, dims = 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+#pragma unroll
+        for (int u = 0; u < KB / 16; u++) {
+            pa_f16x8 ph, pl;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const float a = s[u >> 1][8 * (u & 1) + j], bq = s[u >> 1][8 * (u & 1) + j + 1];
+                const pa_f16x2 hi = __builtin_bit_cast(pa_f16x2, __builtin_amdgcn_cvt_pkrtz(a, bq));
+                ph[j] = hi[0];
+                ph[j + 1] = hi[1];
+                pl[j] = (_Float16)__builtin_fmaf((float)hi[0], -1.0f, a);
+                pl[j + 1] = (_Float16)__builtin_fmaf((float)hi[1], -1.0f, bq);
+            }
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                pa_f16x8 vt[NT];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    pa_s16x4 a[2];
+#pragma unroll
+                    for (int rd = 0; rd < 2; rd++) {
+                        const int kk = 16 * u + 8 * rd + 4 * half + (i >> 2), dd = (32 * d + dims) & (HD - 1);
+                        const int sw = CPR >= 8 ? (kk & 1) << 2 : 0;
+                        char* at = (char*)&vbuf[buf][n][kk * CPR + ((dd >> 3) ^ sw)] + (dd & 4) * 2;
+                        a[rd] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)at);
+                    }
+                    vt[n] = __builtin_bit_cast(pa_f16x8, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vt[0], pl, o[d], 0, 0, 0);
+                if (NT == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vt[NT - 1], ph, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vt[0], ph, o[d], 0, 0, 0);
+            }
+        }
+    };
+
+    // ---- the pipeline: tile it in LDS, it + 1 in registers, the pages of it + 2
+    const int nt = (c1 - c0 + KB - 1) / KB;
+    Raw raw[CK];
+    int page[CK];
+    auto fetch = [&](int it) {                 // tile it from its pages; the pages of tile it + 1
+        const int b = c0 + it * KB;
+#pragma unroll
+        for (int i = 0; i < CK; i++) {
+            load(raw[i], place_of(b + ckey(i), page[i]));
+            page[i] = page_of(b + KB + ckey(i));
+        }
+    };
+    auto put = [&](int it) {
+        if (!stages) return;
+        bool fits = true;
+#pragma unroll
+        for (int i = 0; i < CK; i++) fits &= stage(raw[i], raw[i].in, it & 1, ckey(i), c0 + it * KB + ckey(i));
+        if (!fits) misfit[it & 1] = it;
+    };
+    if (stages) {
+#pragma unroll
+        for (int i = 0; i < CK; i++) page[i] = page_of(c0 + ckey(i));
+    }
+    unsigned long long live = 0;
+    for (int it = -2; it < nt; it++) {
+        const int b = c0 + it * KB, buf = it & 1;
+        const unsigned long long next = it + 1 >= 0 && it + 1 < nt ? live_keys(b + KB) : 0;
+        if (it >= 0) {
+            const bool classes = misfit[buf] == it;      // the same for every wave, and so are the turns below
+            unsigned long long left = live;
+            if (classes) {
+                if (stages)
+#pragma unroll 1
+                    for (int i = 0; i < CK; i++) {
+                        const int key = b + ckey(i);
+                        Raw r;
+                        load(r, place_of(key, page_of(key)));
+                        float y[8];
+                        const unsigned bk = numbers(r.k, r.in, true, key, y), bv = numbers(r.v, r.in, false, key, y);
+                        int ek = bk ? exponent(bk) : 0, ev = exponent(bv);
+                        if (TYPE == KV_I8) {
+                            ek = 0;
+                            ev = exponent(__float_as_uint(scale_of(r.vs, r.in, false, key)) & 0x7fffffffu);
+                        }
+                        if (cc == 0) {
+                            lek[ckey(i)] = ek;
+                            lev[ckey(i)] = ev;
+                        }
+                    }
+                __syncthreads();
+            }
+            do {
+                unsigned long long set = left;
+                if (classes) {
+                    const int k = lane < KB ? lane : 0;
+                    const bool in = lane < KB && (left >> k & 1);
+                    const int ek = in ? lek[k] : 0, ev = in ? lev[k] : 0;
+                    const int mk = pa_wave_max(ek);
+                    const bool in_k = in && (ek == 0 || ek >= mk - PA_BELOW);
+                    const int mv = pa_wave_max(in_k ? ev : 0);
+                    set = __ballot(in_k && ev >= mv - PA_BELOW);
+                    if (mk) EK = mk;
+                    EV = mv;
+                    if (stages)
+#pragma unroll 1
+                        for (int i = 0; i < CK; i++) {
+                            const int key = b + ckey(i);
+                            Raw r;
+                            load(r, place_of(key, page_of(key)));
+                            stage(r, r.in && (set >> ckey(i) & 1), buf, ckey(i), key);
+                        }
+                    __syncthreads();
+                }
+                if (b < wave_hi) compute(buf, b, set);
+                left &= ~set;
+                if (classes) __syncthreads();
+            } while (left);
+        }
+        if (it + 1 >= 0 && it + 1 < nt) put(it + 1);
+        if (stages && it + 2 < nt) fetch(it + 2);
+        live = next;
+        __syncthreads();
+    }
+
+    // ---- out, or this split's part
+    l += __shfl_xor(l, 32, WAVE);
+    if (w0 + (lane & 31) >= R) return;
+    const float nan = __uint_as_float(0x7fc00000u);
+    const bool poor = (qpoor && m != -INFINITY) || kbad < lim;
+    const bool last = keys <= p.chunk_tile;
+    // o to l's reference (in two steps: the power alone may leave fp32's
+    // range), and divided where this is the whole sum
+    const float step = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(0.5f * (mo - (float)PA_W - m));
+    const float inv = step * (last && m != -INFINITY ? 1.0f / l : 1.0f);
+    const long long orow = q0 + tok, slot = (orow * p.heads + head) * p.splits + split;
+    float* dst = last ? p.out + orow * p.ldo + head * HD : p.part_o + slot * HD;
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int d0 = 32 * d + 8 * g + 4 * half;
+            if (d0 < HD) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = poor || bad[d0 + e] < lim ? nan : o[d][4 * g + e] * step * inv;
+                *(f32x4*)(dst + d0) = v;
+            }
+        }
+    if (!last && half == 0) {
+        p.part_ml[2 * slot] = m;
+        p.part_ml[2 * slot + 1] = l;
+    }
+}
+
 // ------------------------------------------------------------------ join
 // out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over a row's splits, in
 // their order; HD / 4 lanes a row.  Sequences of one split are finished already.
@@ -354,10 +881,13 @@ __device__ __forceinline__ void paged_attn_join(const PagedAttnParams& p) {
     if (seq >= c.n || row - qs[seq] >= p.max_q) return;
     const int held = c.kv_len[seq];
     const int keys = held < 0 ? 0 : held > p.max_kv ? p.max_kv : held;
-    if (keys <= p.chunk) return;
+    int qn = c.q_start[seq + 1] - qs[seq];
+    qn = qn < p.max_q ? qn : p.max_q;
+    const int chunk = qn * (p.heads / c.kv_heads) <= p.few_rows ? p.chunk_few : p.chunk_tile;
+    if (keys <= chunk) return;
     int lim = held - (c.q_start[seq + 1] - row) + 1;
     lim = lim < 0 ? 0 : lim > keys ? keys : lim;
-    const int ns = (lim + p.chunk - 1) / p.chunk;
+    const int ns = (lim + chunk - 1) / chunk;
     const long long slot = at * p.splits;
     float m = -INFINITY;
     for (int s = 0; s < ns; s++) m = fmaxf(m, p.part_ml[2 * (slot + s)]);
@@ -376,6 +906,12 @@ __device__ __forceinline__ void paged_attn_join(const PagedAttnParams& p) {
 #define PA_KERNELS(HD, NAME, TYPE)                                                                              \
     extern "C" __global__ void __launch_bounds__(256) k_paged_attn_few_hd##HD##_##NAME(PagedAttnParams p) {     \
         paged_attn_few<HD, TYPE>(p);                                                                            \
+    }                                                                                                           \
+    extern "C" __global__ void __launch_bounds__(256, 2) k_paged_attn_tile4_hd##HD##_##NAME(PagedAttnParams p) { \
+        paged_attn_tile<HD, TYPE, 4, HD == 128 ? 32 : 64>(p);                                                                    \
+    }                                                                                                           \
+    extern "C" __global__ void __launch_bounds__(512, 2) k_paged_attn_tile8_hd##HD##_##NAME(PagedAttnParams p) { \
+        paged_attn_tile<HD, TYPE, 8, HD == 128 ? 32 : 64>(p);                                                                    \
     }
 #define PA_TYPES(HD)                                                                                            \
     PA_KERNELS(HD, f32, KV_F32)                                                                                 \

@@ -18,7 +18,7 @@ struct TrlmServe {
     HipCtx* ctx;
     i32 device;
     /* looked up on first use of a head width and type */
-    hipFunction_t append[NHD][NTYPE][2], read[NHD][NTYPE][2], few[NHD][NTYPE], join[NHD];
+    hipFunction_t append[NHD][NTYPE][2], read[NHD][NTYPE][2], few[NHD][NTYPE], tile[NHD][NTYPE][2], join[NHD];
     hipFunction_t rules[2][2];   /* [narrow, wide][aligned, not] */
 };
 
@@ -183,29 +183,56 @@ i32 trlm_kv_read(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hipDev
 
 /* ---------------- attention ---------------- */
 
-#define FEW_ROWS 16u      /* rows of a k_paged_attn_few workgroup */
+#define FEW_TILE 16u      /* rows of a k_paged_attn_few workgroup */
 #define FEW_KEYS 128u     /* keys its four waves take at a time: splits are multiples of it */
+#define FEW_MAX 32u       /* rows (tokens x group) of a sequence up to which it is taken */
+#define TILE_KEYS 64u     /* keys of a k_paged_attn_tile stage */
 #define FEW_GROUPS 1024u  /* workgroups wanted: four for each of the 256 compute units */
+#define TILE_GROUPS 512u
 #define MAX_SPLITS 256u
 
-typedef struct AttnPlan { u32 tiles, splits, chunk; u64 groups; } AttnPlan;
+typedef struct AttnPlan {
+    u32 few_tiles, tiles, waves;      /* row tiles of a sequence in each kernel (0: not launched) */
+    u32 few_splits, tile_splits, chunk_few, chunk_tile, splits;
+    u64 few_groups, tile_groups;
+} AttnPlan;
 
 static u32 max_kv_of(const TrlmKvCache* c, const TrlmKvSeqs* s) {
     const u64 held = (u64)s->max_pages * c->page_size;
     return s->max_kv > held ? (u32)held : s->max_kv;
 }
 
+/* Splits of kv keys, in multiples of `unit`, so that `groups` row tiles make
+ * at least `wanted` workgroups; returns their number. */
+static u32 split_keys(u32 kv, u64 groups, u32 wanted, u32 unit, u32* chunk) {
+    u64 want = cdiv64(wanted, groups);
+    if (want > MAX_SPLITS) want = MAX_SPLITS;
+    *chunk = (u32)(cdiv64(cdiv64(kv, want), unit) * unit);
+    return (u32)cdiv64(kv, *chunk);
+}
+
 /* A call's launch shape, from what the host knows of it alone, so that a
  * captured call keeps it. */
 static AttnPlan attn_plan(const TrlmKvCache* c, const TrlmKvSeqs* s, u32 heads) {
     AttnPlan p;
-    const u32 group = heads / c->kv_heads, max_q = s->max_q < s->rows ? s->max_q : s->rows, kv = max_kv_of(c, s);
-    p.tiles = (u32)cdiv64((u64)max_q * group, FEW_ROWS);
-    p.groups = (u64)s->n * c->kv_heads * p.tiles;
-    u64 want = p.groups ? cdiv64(FEW_GROUPS, p.groups) : 1;
-    if (want > MAX_SPLITS) want = MAX_SPLITS;
-    p.chunk = (u32)(cdiv64(cdiv64(kv ? kv : 1, want), FEW_KEYS) * FEW_KEYS);
-    p.splits = (u32)cdiv64(kv ? kv : 1, p.chunk);
+    memset(&p, 0, sizeof(p));
+    const u32 group = heads / c->kv_heads, max_q = s->max_q < s->rows ? s->max_q : s->rows;
+    const u32 kv = max_kv_of(c, s) ? max_kv_of(c, s) : 1;
+    const u64 most = (u64)max_q * group, seq_heads = (u64)s->n * c->kv_heads;
+    p.few_tiles = (u32)cdiv64(most < FEW_MAX ? most : FEW_MAX, FEW_TILE);
+    p.few_groups = seq_heads * p.few_tiles;
+    p.few_splits = split_keys(kv, p.few_groups, FEW_GROUPS, FEW_KEYS, &p.chunk_few);
+    p.chunk_tile = p.chunk_few;
+    p.splits = p.few_splits;
+    if (most > FEW_MAX) {
+        p.waves = seq_heads * cdiv64(most, 256) >= 256 ? 8 : 4;
+        p.tiles = (u32)cdiv64(most, 32 * p.waves);
+        p.tile_groups = seq_heads * p.tiles;
+        p.tile_splits = split_keys(kv, p.tile_groups, TILE_GROUPS, TILE_KEYS * 4, &p.chunk_tile);
+        if (p.tile_splits > p.splits) p.splits = p.tile_splits;
+        /* one sequence, or as many rows as all sequences at their longest: none is short */
+        if (s->n == 1 || (u64)s->n * max_q <= s->rows) p.few_splits = 0;
+    }
     return p;
 }
 
@@ -233,7 +260,7 @@ i32 trlm_attn_paged(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hip
     const AttnPlan pl = attn_plan(c, s, heads);
     const u64 need = attn_ws(c, s, heads, &pl);
     if (need && (unaligned(ws, 16) || ws_bytes < need)) return refuse(op, "the workspace is too small or not 16-byte aligned");
-    if (pl.groups > 0x7fffffffull || cdiv64((u64)s->rows * heads, 1024 / hd) > 0x7fffffffull)
+    if (pl.few_groups > 0x7fffffffull || pl.tile_groups > 0x7fffffffull || cdiv64((u64)s->rows * heads, 1024 / hd) > 0x7fffffffull)
         return refuse(op, "too many workgroups");
     PagedAttnParams p;
     memset(&p, 0, sizeof(p));
@@ -244,12 +271,18 @@ i32 trlm_attn_paged(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hip
     p.ldq = (int)ldq; p.ldo = (int)ldo; p.heads = (int)heads;
     p.max_q = (int)(s->max_q < s->rows ? s->max_q : s->rows);
     p.max_kv = (int)max_kv_of(c, s);
-    p.splits = (int)pl.splits; p.chunk = (int)pl.chunk;
+    p.few_rows = (int)FEW_MAX;
+    p.splits = (int)pl.splits; p.chunk_few = (int)pl.chunk_few; p.chunk_tile = (int)pl.chunk_tile;
     p.scale = scale;
     const i32 i = hd_index(hd);
     void* args[] = { &p };
-    hip_launch(kernel_hd(e, &e->few[i][c->type], "k_paged_attn_few", i, (i32)c->type), (u32)pl.groups, pl.splits, 1, 256,
-               1, 1, 0, args);
+    if (pl.tiles)
+        hip_launch(kernel_hd(e, &e->tile[i][c->type][pl.waves == 8], pl.waves == 8 ? "k_paged_attn_tile8" :
+                             "k_paged_attn_tile4", i, (i32)c->type), (u32)pl.tile_groups, pl.tile_splits, 1,
+                   64 * pl.waves, 1, 1, 0, args);
+    if (pl.few_splits)
+        hip_launch(kernel_hd(e, &e->few[i][c->type], "k_paged_attn_few", i, (i32)c->type), (u32)pl.few_groups,
+                   pl.few_splits, 1, 256, 1, 1, 0, args);
     if (pl.splits > 1)
         hip_launch(kernel_hd(e, &e->join[i], "k_paged_attn_join", i, -1),
                    (u32)cdiv64((u64)s->rows * heads, 1024 / hd), 1, 1, 256, 1, 1, 0, args);

@@ -372,15 +372,17 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
 // 4 e + 3 address 16 numbers of row e, and lane j receives number j of rows 0 .. 3.
 typedef _Float16 pa_f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 pa_f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned short pa_u16x2 __attribute__((ext_vector_type(2)));
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pa_s16x4 pa_lds_s16x4;
 
 #define PA_EXP_MIN 12      // rows below 2^-115 take the power of 2^-115 (their scale is then 2^126)
-#define PA_W 14            // a row's weights go up to 2^14
+#define PA_W 10            // a row's weights go up to 2^10, ..
 #define PA_UP 11           // a row's largest magnitude goes to about 2^11 ..
 #define PA_ABOVE 3         // .. and may be up to 2^3 above that
-#define PA_BELOW 6         // .. or 2^6 below
-#define PA_I8_UP 4         // 8-bit integers: times 2^4
+#define PA_BELOW 6         // .. or 2^6 below; together below f16's 2^16
+#define PA_I8_UP 0         // 8-bit integers stay themselves
+#define PA_GROW 4.0f       // a row's maximum may grow by so much (weights to 2^PA_W 2^4) before its sums are rescaled
 
 __device__ __forceinline__ float pa_pow2(int e) {       // 2^e, e kept in [-126, 127]
     e = e < -126 ? -126 : e > 127 ? 127 : e;
@@ -409,9 +411,11 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
     constexpr int CPR = HD / 8, CH = KB * CPR, CK = (CH + THREADS - 1) / THREADS;   // 8-number chunks
     constexpr int NS = HD / 16, DB = (HD + 31) / 32, KT = KB / 32;
     static_assert(KB <= 64 && CH % 64 == 0 && (CH % THREADS == 0 || CH < THREADS), "chunks of whole waves");
-    __shared__ __attribute__((aligned(16))) pa_u32x4 kbuf[2][NT][CH], vbuf[2][NT][CH];
+    constexpr int KLD = HD * 2 + 16;            // bytes of a K row: 16 more keep eight rows' chunks on different banks
+    constexpr int KTERM = KB * KLD, VTERM = KB * HD * 2, BUF = NT * (KTERM + VTERM);
+    __shared__ __attribute__((aligned(16))) char tbuf[2 * BUF];   // two buffers of K terms, then V terms
     __shared__ __attribute__((aligned(16))) float ksc[TYPE == KV_I8 ? 2 : 1][KB], vsc[TYPE == KV_I8 ? 2 : 1][KB];
-    __shared__ int misfit[2], kbad, bad[HD], lek[KB], lev[KB];
+    __shared__ int misfit[2], kbad[64], bad[HD], lek[KB], lev[KB];
     const PagedKv& c = p.kv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int G = p.heads / c.kv_heads;
@@ -449,7 +453,7 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
     const int wave_lo = busy ? limit(w0 / G) : 0, wave_hi = busy ? limit(w1 / G) : 0;
 
     if (threadIdx.x < 2) misfit[threadIdx.x] = -1;
-    if (threadIdx.x == 2) kbad = PA_NONE;
+    if (threadIdx.x < 64) kbad[threadIdx.x] = PA_NONE;
     for (int d = threadIdx.x; d < HD; d += THREADS) bad[d] = PA_NONE;
 
     // operand B of S^T: the row's numbers times scale log2(e), two f16 terms
@@ -522,89 +526,102 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
         }
     };
     int EK = 128, EV = TYPE == KV_I8 ? 124 : 128;   // powers for rows with numbers up to 4 (scales up to 2^-2)
-    // the eight numbers, their row's largest magnitude's bits; what is not
-    // finite becomes 0 and is noted (V: by column, K: by key)
-    auto numbers = [&](const PaRun<TYPE, 8>& run, bool in, bool is_k, int key, float (&y)[8]) -> unsigned {
+    // Eight numbers: the bits of their row's largest magnitude (fp32's, with
+    // zeros below its exponent for bf16).  What is not finite becomes 0 and is
+    // noted (K: the key, by lane; V: the key, by column).
+    auto largest = [&](PaRun<TYPE, 8>& run, bool is_k, int key) -> unsigned {
         unsigned big = 0;
+        if constexpr (TYPE == KV_F32) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            y[e] = in ? run.get(e) : 0.f;
-            if (TYPE != KV_I8) big = max(big, __float_as_uint(y[e]) & 0x7fffffffu);
+            for (int e = 0; e < 8; e++) big = max(big, run.w[e] & 0x7fffffffu);
+        } else if constexpr (TYPE == KV_BF16) {
+            pa_u16x2 two = __builtin_bit_cast(pa_u16x2, run.w[0] & 0x7fff7fffu);
+#pragma unroll
+            for (int e = 1; e < 4; e++)
+                two = __builtin_elementwise_max(two, __builtin_bit_cast(pa_u16x2, run.w[e] & 0x7fff7fffu));
+            const unsigned w = __builtin_bit_cast(unsigned, two);
+            big = max(w & 0xffff0000u, w << 16);
         }
-        if (TYPE != KV_I8) {
-            if (big >= 0x7f800000u) {
-                big = 0;
+        if (TYPE != KV_I8 && big >= 0x7f800000u) {
+            big = 0;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    if ((__float_as_uint(y[e]) & 0x7fffffffu) >= 0x7f800000u) {
-                        if (is_k) atomicMin(&kbad, key);
-                        else atomicMin(&bad[8 * cc + e], key);
-                        y[e] = 0.f;
-                    }
-                    big = max(big, __float_as_uint(y[e]) & 0x7fffffffu);
+            for (int e = 0; e < 8; e++) {
+                const unsigned y = __float_as_uint(run.get(e)) & 0x7fffffffu;
+                if (y >= 0x7f800000u) {
+                    atomicMin(is_k ? &kbad[lane] : &bad[8 * cc + e], key);
+                    if (TYPE == KV_F32) run.w[e] = 0;
+                    if (TYPE == KV_BF16) run.w[e / 2] &= e & 1 ? 0xffffu : 0xffff0000u;
+                } else {
+                    big = max(big, y);
                 }
             }
-            big = pa_row_max<CPR>(big);
         }
-        return big;
+        return pa_row_max<CPR>(big);
     };
     // a row of zeros in K fits any power; in V it has the least one, so that a
     // large weight on it does not stand before the others' contributions
     auto exponent = [](unsigned big) { return max((int)(big >> 23), PA_EXP_MIN); };
     // 8-bit scales: what is not finite as above
-    auto scale_of = [&](float s, bool in, bool is_k, int key) -> float {
-        if (!in) return 0.f;
-        if ((__float_as_uint(s) & 0x7fffffffu) >= 0x7f800000u) {
-            if (is_k) atomicMin(&kbad, key);
-            else
+    auto scale_of = [&](float s, bool is_k, int key) -> float {
+        if ((__float_as_uint(s) & 0x7fffffffu) < 0x7f800000u) return s;
 #pragma unroll
-                for (int e = 0; e < 8; e++) atomicMin(&bad[8 * cc + e], key);
-            return 0.f;
+        for (int e = 0; e < (is_k ? 1 : 8); e++) atomicMin(is_k ? &kbad[lane] : &bad[8 * cc + e], key);
+        return 0.f;
+    };
+    // eight numbers times `up` as f16 terms into LDS, `gap` bytes apart
+    auto terms = [&](const PaRun<TYPE, 8>& run, float up, char* to, int gap) {
+        if constexpr (TYPE == KV_I8) {
+            // byte u of an integer + 128 under 0x64: 1024 + u in f16; less 1152
+            pa_u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const unsigned two = __builtin_amdgcn_perm(0x64646464u, run.w[i / 2] ^ 0x80808080u,
+                                                           i & 1 ? 0x04030402u : 0x04010400u);
+                const pa_f16x2 y = __builtin_bit_cast(pa_f16x2, two) - (pa_f16x2){(_Float16)1152.0f, (_Float16)1152.0f};
+                w[i] = __builtin_bit_cast(unsigned, y);
+            }
+            *(pa_u32x4*)to = w;
+        } else {
+            pa_f16x8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                hi[e] = (_Float16)(run.get(e) * up);
+                if (NT == 2) lo[e] = (_Float16)__builtin_fmaf(run.get(e), up, -(float)hi[e]);
+            }
+            *(pa_u32x4*)to = __builtin_bit_cast(pa_u32x4, hi);
+            if (NT == 2) *(pa_u32x4*)(to + gap) = __builtin_bit_cast(pa_u32x4, lo);
         }
-        return s;
     };
     // one chunk into LDS under the current powers; whether its rows fit them
-    auto stage = [&](const Raw& r, bool in, int buf, int kk, int key) -> bool {
-        float y[8], z[8];
-        const unsigned bk = numbers(r.k, in, true, key, y);
-        const unsigned bv = numbers(r.v, in, false, key, z);
-        bool fits = true;
-        float uk, uv;
+    auto stage = [&](Raw& r, bool in, int buf, int kk, int key) -> bool {
+        if (!in) {
+#pragma unroll
+            for (int i = 0; i < PaRun<TYPE, 8>::NW; i++) r.k.w[i] = r.v.w[i] = 0;     // 8 bits: scales of 0 too
+        }
+        bool fits;
+        float uk = 1.f, uv = 1.f;
         if (TYPE == KV_I8) {
-            const float s = scale_of(r.ks, in, true, key), t = scale_of(r.vs, in, false, key);
+            const float s = in ? scale_of(r.ks, true, key) : 0.f, t = in ? scale_of(r.vs, false, key) : 0.f;
             const int e = exponent(__float_as_uint(t) & 0x7fffffffu);
             fits = !in || (e <= EV && e >= EV - PA_BELOW);
             if (cc == 0) {
                 ksc[buf][kk] = s;
                 vsc[buf][kk] = t * pa_pow2(127 - EV);
             }
-            uk = uv = (float)(1 << PA_I8_UP);
         } else {
+            const unsigned bk = largest(r.k, true, key), bv = largest(r.v, false, key);
             const int a = exponent(bk), b = exponent(bv);
             fits = (bk == 0 || (a <= EK + PA_ABOVE && a >= EK - PA_BELOW)) &&
                    (!in || (b <= EV + PA_ABOVE && b >= EV - PA_BELOW));
             uk = pa_pow2(PA_UP + 127 - EK);
             uv = pa_pow2(PA_UP + 127 - EV);
         }
-        const int swk = CPR >= 8 ? (kk & 7) : CPR == 4 ? ((kk >> 1) & 3) : ((kk >> 2) & 1);
+        // V rows of 128 bytes or more: odd rows have their 64-byte halves
+        // exchanged, so that the transposing reads of four rows meet no bank twice
         const int swv = CPR >= 8 ? (kk & 1) << 2 : 0;
-        pa_f16x8 hi, lo;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float w = y[e] * uk;
-            hi[e] = (_Float16)w;
-            lo[e] = (_Float16)(w - (float)hi[e]);
-        }
-        kbuf[buf][0][kk * CPR + (cc ^ swk)] = __builtin_bit_cast(pa_u32x4, hi);
-        if (NT == 2) kbuf[buf][NT - 1][kk * CPR + (cc ^ swk)] = __builtin_bit_cast(pa_u32x4, lo);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float w = z[e] * uv;
-            hi[e] = (_Float16)w;
-            lo[e] = (_Float16)(w - (float)hi[e]);
-        }
-        vbuf[buf][0][kk * CPR + (cc ^ swv)] = __builtin_bit_cast(pa_u32x4, hi);
-        if (NT == 2) vbuf[buf][NT - 1][kk * CPR + (cc ^ swv)] = __builtin_bit_cast(pa_u32x4, lo);
+        char* at = tbuf + buf * BUF;
+        terms(r.k, uk, at + kk * KLD + 16 * cc, KTERM);
+        terms(r.v, uv, at + NT * KTERM + kk * HD * 2 + 16 * (cc ^ swv), VTERM);
         return fits;
     };
     // the keys of a tile that have a place and are seen by some row
@@ -623,22 +640,27 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
     auto compute = [&](int buf, int b, unsigned long long live) {
         constexpr unsigned long long ALL = KB == 64 ? ~0ull : (1ull << (KB & 63)) - 1;
         f32x16 s[KT];
-        const int r = lane & 31;
+        const char* kt = tbuf + buf * BUF + (lane & 31) * KLD + 16 * half;
+        // operands of four products ahead
+        constexpr int AHEAD = NS < 4 ? NS : 4;
 #pragma unroll
         for (int t = 0; t < KT; t++) {
 #pragma unroll
             for (int e = 0; e < 16; e++) s[t][e] = 0.f;
-            const int kk = 32 * t + r;
-            const int sw = CPR >= 8 ? (kk & 7) : CPR == 4 ? ((kk >> 1) & 3) : ((kk >> 2) & 1);
 #pragma unroll
-            for (int n = 0; n < NS; n++) {
-                const pa_f16x8 kh = __builtin_bit_cast(pa_f16x8, kbuf[buf][0][kk * CPR + ((2 * n + half) ^ sw)]);
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[n], s[t], 0, 0, 0);
-                if (NT == 2) {
-                    const pa_f16x8 kl = __builtin_bit_cast(pa_f16x8, kbuf[buf][NT - 1][kk * CPR + ((2 * n + half) ^ sw)]);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[n], s[t], 0, 0, 0);
+            for (int n0 = 0; n0 < NS; n0 += AHEAD) {
+                pa_f16x8 kf[AHEAD][NT];
+#pragma unroll
+                for (int n = 0; n < AHEAD; n++)
+#pragma unroll
+                    for (int w = 0; w < NT; w++)
+                        kf[n][w] = *(const pa_f16x8*)(kt + w * KTERM + 32 * t * KLD + 32 * (n0 + n));
+#pragma unroll
+                for (int n = 0; n < AHEAD; n++) {
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][0], ql[n0 + n], s[t], 0, 0, 0);
+                    if (NT == 2) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][NT - 1], qh[n0 + n], s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][0], qh[n0 + n], s[t], 0, 0, 0);
                 }
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[n], s[t], 0, 0, 0);
             }
             if (TYPE == KV_I8) {
 #pragma unroll
@@ -669,13 +691,21 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
 #pragma unroll
             for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(s[t][e], s[t][e + 1]));
         top = fmaxf(top, __shfl_xor(top, 32, WAVE)) * cu;
-        // (a row that has seen no key yet: references of 0, and zeros)
-        const float mo_new = fmaxf(mo, top + ev), m_new = fmaxf(m, top);
-        const float ref = m_new == -INFINITY ? 0.f : m_new, refo = m_new == -INFINITY ? 0.f : mo_new;
-        const float alpha = __builtin_amdgcn_exp2f(mo - refo);
-        l *= __builtin_amdgcn_exp2f(m - ref);
-        m = m_new;
-        mo = mo_new;
+        // The references m and mo follow the maxima only when one of the wave's
+        // rows has outgrown its own (a row that has seen no key yet: references
+        // of 0, and zeros).
+        if (__ballot(top > m + PA_GROW || top + ev > mo + PA_GROW)) {
+            const float m_new = fmaxf(m, top), mo_new = fmaxf(mo, top + ev);
+            const float alpha = mo_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mo - mo_new);
+            l *= m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            mo = mo_new;
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= alpha;
+        }
+        const float ref = m == -INFINITY ? 0.f : m, refo = mo == -INFINITY ? 0.f : mo;
         // a weight 2^(s - ref) is 2^gap of the same key's 2^(s + ev - refo + W)
         const float off = (float)PA_W + ev - refo, gap = -off - ref;
         const bool far = __ballot(gap > 60.0f) != 0;
@@ -708,13 +738,11 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
             }
         }
         if (!far) l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(gap), l);
-        if (__ballot(alpha != 1.0f)) {
-#pragma unroll
-            for (int d = 0; d < DB; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) o[d][e] *= alpha;
-        }
-        const int i = lane & 15, dims = 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+        const int i = lane & 15, p_ = CPR >= 8 ? (i >> 2) & 1 : 0;
+        const int dims = (16 * ((lane >> 4) & 1) + 4 * (i & 3)) & (HD - 1);
+        const char* vt = tbuf + buf * BUF + NT * KTERM + (4 * half + (i >> 2)) * HD * 2 + dims * 2;
+        float minus = -1.0f;
+        asm("" : "+s"(minus));      // kept a factor: v_fma_mix takes the f16 term as it is
 #pragma unroll
         for (int u = 0; u < KB / 16; u++) {
             pa_f16x8 ph, pl;
@@ -724,27 +752,26 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
                 const pa_f16x2 hi = __builtin_bit_cast(pa_f16x2, __builtin_amdgcn_cvt_pkrtz(a, bq));
                 ph[j] = hi[0];
                 ph[j + 1] = hi[1];
-                pl[j] = (_Float16)__builtin_fmaf((float)hi[0], -1.0f, a);
-                pl[j + 1] = (_Float16)__builtin_fmaf((float)hi[1], -1.0f, bq);
+                pl[j] = (_Float16)__builtin_fmaf((float)hi[0], minus, a);
+                pl[j + 1] = (_Float16)__builtin_fmaf((float)hi[1], minus, bq);
             }
+            pa_f16x8 vf[DB][NT];
 #pragma unroll
-            for (int d = 0; d < DB; d++) {
-                pa_f16x8 vt[NT];
+            for (int d = 0; d < DB; d++)
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     pa_s16x4 a[2];
 #pragma unroll
-                    for (int rd = 0; rd < 2; rd++) {
-                        const int kk = 16 * u + 8 * rd + 4 * half + (i >> 2), dd = (32 * d + dims) & (HD - 1);
-                        const int sw = CPR >= 8 ? (kk & 1) << 2 : 0;
-                        char* at = (char*)&vbuf[buf][n][kk * CPR + ((dd >> 3) ^ sw)] + (dd & 4) * 2;
-                        a[rd] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pa_lds_s16x4*)at);
-                    }
-                    vt[n] = __builtin_bit_cast(pa_f16x8, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    for (int rd = 0; rd < 2; rd++)
+                        a[rd] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (pa_lds_s16x4*)(vt + n * VTERM + (16 * u + 8 * rd) * HD * 2 + 64 * (d ^ p_)));
+                    vf[d][n] = __builtin_bit_cast(pa_f16x8, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
                 }
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vt[0], pl, o[d], 0, 0, 0);
-                if (NT == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vt[NT - 1], ph, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vt[0], ph, o[d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d][0], pl, o[d], 0, 0, 0);
+                if (NT == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d][NT - 1], ph, o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d][0], ph, o[d], 0, 0, 0);
             }
         }
     };
@@ -786,12 +813,13 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
                         const int key = b + ckey(i);
                         Raw r;
                         load(r, place_of(key, page_of(key)));
-                        float y[8];
-                        const unsigned bk = numbers(r.k, r.in, true, key, y), bv = numbers(r.v, r.in, false, key, y);
-                        int ek = bk ? exponent(bk) : 0, ev = exponent(bv);
-                        if (TYPE == KV_I8) {
-                            ek = 0;
-                            ev = exponent(__float_as_uint(scale_of(r.vs, r.in, false, key)) & 0x7fffffffu);
+                        int ek = 0, ev = PA_EXP_MIN;
+                        if (r.in && TYPE == KV_I8) {
+                            ev = exponent(__float_as_uint(scale_of(r.vs, false, key)) & 0x7fffffffu);
+                        } else if (r.in) {
+                            const unsigned bk = largest(r.k, true, key);
+                            ek = bk ? exponent(bk) : 0;
+                            ev = exponent(largest(r.v, false, key));
                         }
                         if (cc == 0) {
                             lek[ckey(i)] = ek;
@@ -835,9 +863,12 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
 
     // ---- out, or this split's part
     l += __shfl_xor(l, 32, WAVE);
+    int kfirst = kbad[lane];
+#pragma unroll
+    for (int f = 32; f >= 1; f >>= 1) kfirst = min(kfirst, __shfl_xor(kfirst, f, WAVE));
     if (w0 + (lane & 31) >= R) return;
     const float nan = __uint_as_float(0x7fc00000u);
-    const bool poor = (qpoor && m != -INFINITY) || kbad < lim;
+    const bool poor = (qpoor && m != -INFINITY) || kfirst < lim;
     const bool last = keys <= p.chunk_tile;
     // o to l's reference (in two steps: the power alone may leave fp32's
     // range), and divided where this is the whole sum

@@ -185,7 +185,7 @@ i32 trlm_kv_read(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hipDev
 
 #define FEW_TILE 16u      /* rows of a k_paged_attn_few workgroup */
 #define FEW_KEYS 128u     /* keys its four waves take at a time: splits are multiples of it */
-#define FEW_MAX 32u       /* rows (tokens x group) of a sequence up to which it is taken */
+#define FEW_MAX 64u       /* rows (tokens x group) of a sequence up to which it is taken */
 #define TILE_KEYS 64u     /* keys of a k_paged_attn_tile stage */
 #define FEW_GROUPS 1024u  /* workgroups wanted: four for each of the 256 compute units */
 #define TILE_GROUPS 512u

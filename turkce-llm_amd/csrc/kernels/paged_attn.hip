@@ -415,7 +415,8 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
     constexpr int KTERM = KB * KLD, VTERM = KB * HD * 2, BUF = NT * (KTERM + VTERM);
     __shared__ __attribute__((aligned(16))) char tbuf[2 * BUF];   // two buffers of K terms, then V terms
     __shared__ __attribute__((aligned(16))) float ksc[TYPE == KV_I8 ? 2 : 1][KB], vsc[TYPE == KV_I8 ? 2 : 1][KB];
-    __shared__ int misfit[2], kbad[64], bad[HD], lek[KB], lev[KB];
+    __shared__ int misfit[2], kbad[64], lek[KB], lev[KB];
+    __shared__ __attribute__((aligned(16))) int bad[HD];
     const PagedKv& c = p.kv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int G = p.heads / c.kv_heads;
@@ -624,29 +625,36 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
         terms(r.v, uv, at + NT * KTERM + kk * HD * 2 + 16 * (cc ^ swv), VTERM);
         return fits;
     };
-    // the keys of a tile that have a place and are seen by some row
-    auto live_keys = [&](int b) -> unsigned long long {
+    // The keys of a tile that have a place and are seen by some row, from the
+    // pages of its 16-key groups that lanes 0 .. KB / 16 - 1 hold.  (Read with
+    // the vector loads: a scalar load in flight would make every wait for an
+    // LDS read wait for it too.)
+    auto live_keys = [&](int b, int page) -> unsigned long long {
+        const unsigned groups = (unsigned)__ballot(page >= 0 && page < c.num_pages);
         unsigned long long live = 0;
 #pragma unroll
-        for (int g = 0; g < KB / 16; g++) {
-            const int page = page_of(b + 16 * g);
-            if (page >= 0 && page < c.num_pages) live |= 0xffffull << (16 * g);
-        }
+        for (int g = 0; g < KB / 16; g++)
+            if (groups >> g & 1) live |= 0xffffull << (16 * g);
         const int left = c1 - b;
         return left >= 64 ? live : live & ((1ull << (left > 0 ? left : 0)) - 1);
     };
 
-    // ---- one tile of LDS into this wave's rows
+    // ---- one tile of LDS into this wave's rows, 32 keys at a time: the score
+    // products of the next 32 keys run beside the exponentials of these
     auto compute = [&](int buf, int b, unsigned long long live) {
         constexpr unsigned long long ALL = KB == 64 ? ~0ull : (1ull << (KB & 63)) - 1;
-        f32x16 s[KT];
         const char* kt = tbuf + buf * BUF + (lane & 31) * KLD + 16 * half;
-        // operands of four products ahead
-        constexpr int AHEAD = NS < 4 ? NS : 4;
+        const int i = lane & 15, p_ = CPR >= 8 ? (i >> 2) & 1 : 0;
+        const int dims = (16 * ((lane >> 4) & 1) + 4 * (i & 3)) & (HD - 1);
+        const char* vt = tbuf + buf * BUF + NT * KTERM + (4 * half + (i >> 2)) * HD * 2 + dims * 2;
+        const float cu = pa_pow2(qe + (TYPE == KV_I8 ? -PA_I8_UP : EK - 127 - PA_UP));
+        const float ev = (float)(EV - 127 - (TYPE == KV_I8 ? PA_I8_UP : PA_UP));
+        float minus = -1.0f;
+        asm("" : "+s"(minus));      // kept a factor: v_fma_mix takes the f16 term as it is
+        auto scores = [&](int t, f32x16& s) {
+            constexpr int AHEAD = NS < 4 ? NS : 4;      // operands of four products ahead
 #pragma unroll
-        for (int t = 0; t < KT; t++) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[t][e] = 0.f;
+            for (int e = 0; e < 16; e++) s[e] = 0.f;
 #pragma unroll
             for (int n0 = 0; n0 < NS; n0 += AHEAD) {
                 pa_f16x8 kf[AHEAD][NT];
@@ -657,121 +665,114 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
                         kf[n][w] = *(const pa_f16x8*)(kt + w * KTERM + 32 * t * KLD + 32 * (n0 + n));
 #pragma unroll
                 for (int n = 0; n < AHEAD; n++) {
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][0], ql[n0 + n], s[t], 0, 0, 0);
-                    if (NT == 2) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][NT - 1], qh[n0 + n], s[t], 0, 0, 0);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][0], qh[n0 + n], s[t], 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][0], ql[n0 + n], s, 0, 0, 0);
+                    if (NT == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][NT - 1], qh[n0 + n], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n][0], qh[n0 + n], s, 0, 0, 0);
                 }
             }
+        };
+        f32x16 ss[KT];
+        scores(0, ss[0]);
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+            f32x16& s = ss[t];
             if (TYPE == KV_I8) {
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
                     const f32x4 f = *(const f32x4*)&ksc[buf][32 * t + 8 * g + 4 * half];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[t][4 * g + e] *= f[e];
+                    for (int e = 0; e < 4; e++) s[4 * g + e] *= f[e];
                 }
             }
-        }
-        if (live != ALL || b + KB > wave_lo) {
-            const int seen = lim - b - 4 * half;
+            if (live != ALL || b + KB > wave_lo) {
+                // bit kk: this lane's key 8 (e / 4) + e % 4 = kk is seen and held
+                const int seen = lim - b - 4 * half - 32 * t;
+                unsigned held_here = (unsigned)(live >> (32 * t)) >> (4 * half);
+                held_here &= seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1;
+                asm("" : "+v"(held_here));      // (the tests below stay in this branch)
 #pragma unroll
-            for (int t = 0; t < KT; t++) {
-                const unsigned lt = (unsigned)(live >> (32 * t)) >> (4 * half);
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int kk = 8 * (e >> 2) + (e & 3);
-                    if (32 * t + kk >= seen || !(lt >> kk & 1)) s[t][e] = -INFINITY;
-                }
+                for (int e = 0; e < 16; e++)
+                    if (!(held_here >> (8 * (e >> 2) + (e & 3)) & 1)) s[e] = -INFINITY;
             }
-        }
-        const float cu = pa_pow2(qe + (TYPE == KV_I8 ? -PA_I8_UP : EK - 127 - PA_UP));
-        const float ev = (float)(EV - 127 - (TYPE == KV_I8 ? PA_I8_UP : PA_UP));
-        float top = -INFINITY;
+            float top = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < KT; t++)
+            for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(s[e], s[e + 1]));
+            {
+                const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * cu;
+            }
+            // The references m and mo follow the maxima only when one of the
+            // wave's rows has outgrown its own (a row that has seen no key yet:
+            // references of 0, and zeros).
+            if (__ballot(top > m + PA_GROW || top + ev > mo + PA_GROW)) {
+                const float m_new = fmaxf(m, top), mo_new = fmaxf(mo, top + ev);
+                const float alpha = mo_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mo - mo_new);
+                l *= m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+                m = m_new;
+                mo = mo_new;
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(s[t][e], s[t][e + 1]));
-        top = fmaxf(top, __shfl_xor(top, 32, WAVE)) * cu;
-        // The references m and mo follow the maxima only when one of the wave's
-        // rows has outgrown its own (a row that has seen no key yet: references
-        // of 0, and zeros).
-        if (__ballot(top > m + PA_GROW || top + ev > mo + PA_GROW)) {
-            const float m_new = fmaxf(m, top), mo_new = fmaxf(mo, top + ev);
-            const float alpha = mo_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mo - mo_new);
-            l *= m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-            m = m_new;
-            mo = mo_new;
+                for (int d = 0; d < DB; d++)
 #pragma unroll
-            for (int d = 0; d < DB; d++)
+                    for (int e = 0; e < 16; e++) o[d][e] *= alpha;
+            }
+            const float ref = m == -INFINITY ? 0.f : m, refo = mo == -INFINITY ? 0.f : mo;
+            // a weight 2^(s - ref) is 2^gap of the same key's 2^(s + ev - refo + W)
+            const float off = (float)PA_W + ev - refo, gap = -off - ref;
+            float part = 1.0f;
+            if (__ballot(gap > 60.0f)) {
+                // values so much smaller than another key's that their weights
+                // would leave fp32's range beside it: summed on their own
+                part = 0.f;
 #pragma unroll
-                for (int e = 0; e < 16; e++) o[d][e] *= alpha;
-        }
-        const float ref = m == -INFINITY ? 0.f : m, refo = mo == -INFINITY ? 0.f : mo;
-        // a weight 2^(s - ref) is 2^gap of the same key's 2^(s + ev - refo + W)
-        const float off = (float)PA_W + ev - refo, gap = -off - ref;
-        const bool far = __ballot(gap > 60.0f) != 0;
-        float sum = 0.f;
-        if (far) {
-            // values so much smaller than another key's that their weights
-            // would leave fp32's range beside it: summed on their own
-#pragma unroll
-            for (int t = 0; t < KT; t++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], cu, -ref));
-            l += sum;
-        }
-        sum = 0.f;
-#pragma unroll
-        for (int t = 0; t < KT; t++) {
+                for (int e = 0; e < 16; e++) l += __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], cu, -ref));
+            }
+            if (t + 1 < KT) scores(t + 1, ss[t + 1 < KT ? t + 1 : t]);
+            pa_f16x8 ph[2], pl[2];
+            float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], cu, off));
-                sum += w;
-                s[t][e] = w;
+                s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], cu, off));
+                sum[e & 1] += s[e];
             }
             if (TYPE == KV_I8) {
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
                     const f32x4 f = *(const f32x4*)&vsc[buf][32 * t + 8 * g + 4 * half];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[t][4 * g + e] *= f[e];
+                    for (int e = 0; e < 4; e++) s[4 * g + e] *= f[e];
                 }
             }
-        }
-        if (!far) l = __builtin_fmaf(sum, __builtin_amdgcn_exp2f(gap), l);
-        const int i = lane & 15, p_ = CPR >= 8 ? (i >> 2) & 1 : 0;
-        const int dims = (16 * ((lane >> 4) & 1) + 4 * (i & 3)) & (HD - 1);
-        const char* vt = tbuf + buf * BUF + NT * KTERM + (4 * half + (i >> 2)) * HD * 2 + dims * 2;
-        float minus = -1.0f;
-        asm("" : "+s"(minus));      // kept a factor: v_fma_mix takes the f16 term as it is
 #pragma unroll
-        for (int u = 0; u < KB / 16; u++) {
-            pa_f16x8 ph, pl;
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                const float a = s[u >> 1][8 * (u & 1) + j], bq = s[u >> 1][8 * (u & 1) + j + 1];
-                const pa_f16x2 hi = __builtin_bit_cast(pa_f16x2, __builtin_amdgcn_cvt_pkrtz(a, bq));
-                ph[j] = hi[0];
-                ph[j + 1] = hi[1];
-                pl[j] = (_Float16)__builtin_fmaf((float)hi[0], minus, a);
-                pl[j + 1] = (_Float16)__builtin_fmaf((float)hi[1], minus, bq);
-            }
-            pa_f16x8 vf[DB][NT];
-#pragma unroll
-            for (int d = 0; d < DB; d++)
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    pa_s16x4 a[2];
-#pragma unroll
-                    for (int rd = 0; rd < 2; rd++)
-                        a[rd] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (pa_lds_s16x4*)(vt + n * VTERM + (16 * u + 8 * rd) * HD * 2 + 64 * (d ^ p_)));
-                    vf[d][n] = __builtin_bit_cast(pa_f16x8, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                for (int j = 0; j < 8; j += 2) {
+                    const pa_f16x2 hi = __builtin_bit_cast(pa_f16x2, __builtin_amdgcn_cvt_pkrtz(s[8 * u + j], s[8 * u + j + 1]));
+                    ph[u][j] = hi[0];
+                    ph[u][j + 1] = hi[1];
+                    pl[u][j] = (_Float16)__builtin_fmaf((float)hi[0], minus, s[8 * u + j]);
+                    pl[u][j + 1] = (_Float16)__builtin_fmaf((float)hi[1], minus, s[8 * u + j + 1]);
                 }
+            l = __builtin_fmaf(sum[0] + sum[1], part * __builtin_amdgcn_exp2f(fminf(gap, 100.0f)), l);
 #pragma unroll
-            for (int d = 0; d < DB; d++) {
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d][0], pl, o[d], 0, 0, 0);
-                if (NT == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d][NT - 1], ph, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d][0], ph, o[d], 0, 0, 0);
+            for (int u = 0; u < 2; u++) {
+                pa_f16x8 vf[DB][NT];
+#pragma unroll
+                for (int d = 0; d < DB; d++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        pa_s16x4 a[2];
+#pragma unroll
+                        for (int rd = 0; rd < 2; rd++)
+                            a[rd] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (pa_lds_s16x4*)(vt + n * VTERM + (32 * t + 16 * u + 8 * rd) * HD * 2 + 64 * (d ^ p_)));
+                        vf[d][n] = __builtin_bit_cast(pa_f16x8, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    }
+#pragma unroll
+                for (int d = 0; d < DB; d++) {
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d][0], pl[u], o[d], 0, 0, 0);
+                    if (NT == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d][NT - 1], ph[u], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d][0], ph[u], o[d], 0, 0, 0);
+                }
             }
         }
     };
@@ -799,11 +800,12 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
 #pragma unroll
         for (int i = 0; i < CK; i++) page[i] = page_of(c0 + ckey(i));
     }
-    unsigned long long live = 0;
+    int group_page = page_of(c0 + 16 * (lane & (KB / 16 - 1)));
     for (int it = -2; it < nt; it++) {
         const int b = c0 + it * KB, buf = it & 1;
-        const unsigned long long next = it + 1 >= 0 && it + 1 < nt ? live_keys(b + KB) : 0;
         if (it >= 0) {
+            const unsigned long long live = live_keys(b, group_page);
+            group_page = page_of(b + KB + 16 * (lane & (KB / 16 - 1)));
             const bool classes = misfit[buf] == it;      // the same for every wave, and so are the turns below
             unsigned long long left = live;
             if (classes) {
@@ -857,7 +859,6 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
         }
         if (it + 1 >= 0 && it + 1 < nt) put(it + 1);
         if (stages && it + 2 < nt) fetch(it + 2);
-        live = next;
         __syncthreads();
     }
 
@@ -882,9 +883,11 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
         for (int g = 0; g < 4; g++) {
             const int d0 = 32 * d + 8 * g + 4 * half;
             if (d0 < HD) {
+                const int4 first = *(const int4*)&bad[d0];
+                const int fe[4] = {first.x, first.y, first.z, first.w};
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = poor || bad[d0 + e] < lim ? nan : o[d][4 * g + e] * step * inv;
+                for (int e = 0; e < 4; e++) v[e] = poor | (fe[e] < lim) ? nan : o[d][4 * g + e] * step * inv;
                 *(f32x4*)(dst + d0) = v;
             }
         }
@@ -942,7 +945,7 @@ __device__ __forceinline__ void paged_attn_join(const PagedAttnParams& p) {
         paged_attn_tile<HD, TYPE, 4, HD == 128 ? 32 : 64>(p);                                                                    \
     }                                                                                                           \
     extern "C" __global__ void __launch_bounds__(512, 2) k_paged_attn_tile8_hd##HD##_##NAME(PagedAttnParams p) { \
-        paged_attn_tile<HD, TYPE, 8, HD == 128 ? 32 : 64>(p);                                                                    \
+        paged_attn_tile<HD, TYPE, 8, HD == 128 && TYPE == KV_F32 ? 32 : 64>(p);                                                                    \
     }
 #define PA_TYPES(HD)                                                                                            \
     PA_KERNELS(HD, f32, KV_F32)                                                                                 \

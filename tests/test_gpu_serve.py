@@ -486,7 +486,7 @@ def test_rules_sizes(trlm, box, V, pad, in_place):
     rules_case(trlm, box, rng, 3, V, 40, 6, True, pad, in_place)
 
 
-@pytest.mark.parametrize("rows,V", [(70, 31769), (130, 20001)])
+@pytest.mark.parametrize("rows,V", [(70, 31769), (1030, 16001)])
 def test_rules_many_rows(trlm, box, rows, V):
     """Enough rows for the wide slices, aligned and not."""
     rng = np.random.default_rng(rows)

@@ -50,6 +50,25 @@ __device__ __forceinline__ void logits_rules(const RulesParams& p) {
         }
     }
     if (p.history || p.bias_ids) {
+        // the first ids of the row, as far as its memory goes: in flight before
+        // their number is known
+        constexpr int AHEAD = 4;
+        unsigned id[AHEAD], bid = 0;
+        const unsigned* hist = p.history + row * p.ld_hist;
+        const unsigned* ids = p.bias_ids + row * p.ld_bias;
+        int len = 0, gen = 0, n = 0;
+        if (p.history) {
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++) id[a] = t + a * THREADS < p.ld_hist ? hist[t + a * THREADS] : 0;
+            len = p.hist_len[row];
+            len = len < 0 ? 0 : len > p.ld_hist ? (int)p.ld_hist : len;
+            if (p.gen_start) gen = p.gen_start[row];
+        }
+        if (p.bias_ids) {
+            if (t < p.ld_bias) bid = ids[t];
+            n = p.n_bias[row];
+            n = n < 0 ? 0 : n > p.ld_bias ? (int)p.ld_bias : n;
+        }
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int at = 4 * (t + i * THREADS);
@@ -57,28 +76,25 @@ __device__ __forceinline__ void logits_rules(const RulesParams& p) {
             *(int4*)(bias_at + at) = make_int4(-1, -1, -1, -1);
         }
         __syncthreads();
+        auto count = [&](unsigned k, int j) {
+            k -= (unsigned)t0;
+            if (k < (unsigned)left) {
+                atomicOr(seen + k, 1u);
+                if (j >= gen) atomicAdd(seen + k, 2u);
+            }
+        };
         if (p.history) {
-            const unsigned* hist = p.history + row * p.ld_hist;
-            int len = p.hist_len[row];
-            len = len < 0 ? 0 : len > p.ld_hist ? (int)p.ld_hist : len;
-            const int gen = p.gen_start ? p.gen_start[row] : 0;
-            for (int j = t; j < len; j += THREADS) {
-                const unsigned k = hist[j] - (unsigned)t0;
-                if (k < (unsigned)left) {
-                    atomicOr(seen + k, 1u);
-                    if (j >= gen) atomicAdd(seen + k, 2u);
-                }
-            }
+#pragma unroll
+            for (int a = 0; a < AHEAD; a++)
+                if (t + a * THREADS < len) count(id[a], t + a * THREADS);
+            for (int j = t + AHEAD * THREADS; j < len; j += THREADS) count(hist[j], j);
         }
-        if (p.bias_ids) {
-            const unsigned* ids = p.bias_ids + row * p.ld_bias;
-            int n = p.n_bias[row];
-            n = n < 0 ? 0 : n > p.ld_bias ? (int)p.ld_bias : n;
-            for (int j = t; j < n; j += THREADS) {
-                const unsigned k = ids[j] - (unsigned)t0;
-                if (k < (unsigned)left) atomicMax(bias_at + k, j);
-            }
-        }
+        auto place = [&](unsigned k, int j) {
+            k -= (unsigned)t0;
+            if (k < (unsigned)left) atomicMax(bias_at + k, j);
+        };
+        if (t < n) place(bid, t);
+        for (int j = t + THREADS; j < n; j += THREADS) place(ids[j], j);
         __syncthreads();
     }
     const bool edit = p.history || p.bias_ids;

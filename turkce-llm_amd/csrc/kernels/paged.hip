@@ -54,27 +54,47 @@ __device__ __forceinline__ long long paged_place(const PagedKv& c, int seq, int 
 // then once to fp32: the same bits in any order of operations, which the 8-bit
 // form needs (a last-bit difference next to a step's border is a whole step).
 // The 64-bit arithmetic is hidden behind the memory.
-__device__ __forceinline__ void paged_turn(float& x0, float& x1, float c, float s) {
-    const double a = x0, b = x1, cd = c, sd = s;
-    x0 = (float)(a * cd - b * sd);
-    x1 = (float)(a * sd + b * cd);
+__device__ __forceinline__ void paged_turn(float& x0, float& x1, double c, double s) {
+    const double a = x0, b = x1;
+    x0 = (float)(a * c - b * s);
+    x1 = (float)(a * s + b * c);
 }
 
-// The four numbers of lane c4 (columns 4 c4 .. + 3 of its head) turned by the
-// angles at `row` of the tables.  Half layout: a column's partner is rot / 2
-// away, in the lane rot / 8 away (rot % 8 == 0), fetched by a shuffle in which
-// the whole wave takes part.
-__device__ __forceinline__ f32x4 paged_rope(const KvAppendParams& p, f32x4 x, int pos, int c4, bool turn) {
-    if (!p.rot_half) {
-        if (turn && 4 * c4 < p.rot) {
-            const long long t = (long long)pos * (p.rot >> 1) + 2 * c4;
-            const pg_f32x2 c = *(const pg_f32x2*)(p.cos_t + t), s = *(const pg_f32x2*)(p.sin_t + t);
-            float a = x[0], b = x[1], d = x[2], e = x[3];
-            paged_turn(a, b, c[0], s[0]);
-            paged_turn(d, e, c[1], s[1]);
-            x = f32x4{a, b, d, e};
+// The angles of lane c4's numbers (columns 4 c4 .. + 3 of a head) at `pos`, in
+// 64 bits: two pairs' in the interleaved layout, four in the half layout, whose
+// columns i and i + rot / 2 share row i of the tables.
+struct PagedAngles {
+    double c[4], s[4];
+    __device__ __forceinline__ void load(const KvAppendParams& p, int pos, int c4) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) c[e] = s[e] = 0;
+        if (!p.rot) return;
+        const int far = p.rot >> 3;
+        const long long t = (long long)pos * (p.rot >> 1) + (p.rot_half ? 4 * (c4 < far ? c4 : c4 - far) : 2 * c4);
+        if (p.rot_half) {
+            const f32x4 x = *(const f32x4*)(p.cos_t + t), y = *(const f32x4*)(p.sin_t + t);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                c[e] = x[e];
+                s[e] = y[e];
+            }
+        } else {
+            const pg_f32x2 x = *(const pg_f32x2*)(p.cos_t + t), y = *(const pg_f32x2*)(p.sin_t + t);
+            c[0] = x[0]; c[1] = x[1];
+            s[0] = y[0]; s[1] = y[1];
         }
-        return x;
+    }
+};
+
+// Four numbers turned.  Half layout: a column's partner is rot / 2 away, in the
+// lane rot / 8 away (rot % 8 == 0), fetched by a shuffle in which the whole wave
+// takes part.
+__device__ __forceinline__ f32x4 paged_rope(const KvAppendParams& p, f32x4 x, const PagedAngles& t, int c4, bool turn) {
+    if (!p.rot_half) {
+        float a = x[0], b = x[1], d = x[2], e = x[3];
+        paged_turn(a, b, t.c[0], t.s[0]);
+        paged_turn(d, e, t.c[1], t.s[1]);
+        return turn ? f32x4{a, b, d, e} : x;
     }
     const int far = p.rot >> 3, lane = threadIdx.x & 63;
     const bool low = c4 < far, in = 4 * c4 < p.rot;
@@ -82,17 +102,13 @@ __device__ __forceinline__ f32x4 paged_rope(const KvAppendParams& p, f32x4 x, in
     f32x4 y;
 #pragma unroll
     for (int e = 0; e < 4; e++) y[e] = __shfl(x[e], from, WAVE);
-    if (turn && in) {
-        const int i = 4 * (low ? c4 : c4 - far);
-        const long long t = (long long)pos * (p.rot >> 1) + i;
-        const f32x4 c = *(const f32x4*)(p.cos_t + t), s = *(const f32x4*)(p.sin_t + t);
+    if (turn)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            float a = low ? x[e] : y[e], b = low ? y[e] : x[e];
-            paged_turn(a, b, c[e], s[e]);
-            x[e] = low ? a : b;
+            // low columns: x cos - y sin; high ones: y sin + x cos
+            const double xd = x[e], yd = y[e];
+            x[e] = (float)(low ? xd * t.c[e] - yd * t.s[e] : yd * t.s[e] + xd * t.c[e]);
         }
-    }
     return x;
 }
 
@@ -133,81 +149,80 @@ __device__ __forceinline__ void paged_store(void* pool, float* scales, long long
     }
 }
 
-// One head (blockIdx.y: the query heads, then the key heads, then the value
-// heads) of U * 256 / LPR consecutive rows per workgroup, LPR = HD / 4 lanes a
-// row: a row's numbers are read as one run, and consecutive tokens of a
-// sequence write consecutive cache rows.  All U loads are in flight before the
-// first use.
+// U heads (blockIdx.y: of the query heads, then the key heads, then the value
+// heads) of 256 / LPR consecutive rows per workgroup, LPR = HD / 4 lanes a row: a
+// row's numbers of a head are read as one run, consecutive tokens of a sequence
+// write consecutive cache rows, and a row's place and angles are found once for
+// its U heads.  All U loads are in flight before the first use.
 template <int HD, int TYPE, int U>
 __device__ __forceinline__ void kv_append(const KvAppendParams& p) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR;
     __shared__ int qs[PAGED_MAX_SEQS + 1];
-    const int c4 = threadIdx.x % LPR, sub = threadIdx.x / LPR;
-    const int head = blockIdx.y;
-    const int kh = p.kv.kv_heads;
-    const int kind = head < p.heads ? 0 : head < p.heads + kh ? 1 : 2;
-    const int h = kind == 0 ? head : kind == 1 ? head - p.heads : head - p.heads - kh;
-    const float* src = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
-    const long long ld = kind == 0 ? p.ldq : kind == 1 ? p.ldk : p.ldv;
-    const int row0 = blockIdx.x * (RPB * U) + sub;
+    const int c4 = threadIdx.x % LPR;
+    const int row = blockIdx.x * RPB + threadIdx.x / LPR;
+    const long long at_row = row < p.kv.rows ? row : 0;
+    const int kh = p.kv.kv_heads, all = p.heads + 2 * kh;
     f32x4 x[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int row = row0 + u * RPB;
-        x[u] = *(const f32x4*)(src + (long long)(row < p.kv.rows ? row : 0) * ld + h * HD + 4 * c4);
+        const int head = blockIdx.y * U + u < all ? blockIdx.y * U + u : all - 1;
+        const float* src = head < p.heads ? p.q + at_row * p.ldq + head * HD
+                           : head < p.heads + kh ? p.k + at_row * p.ldk + (head - p.heads) * HD
+                                                 : p.v + at_row * p.ldv + (head - p.heads - kh) * HD;
+        x[u] = *(const f32x4*)(src + 4 * c4);
     }
     paged_stage_starts(p.kv, qs);
+    const int seq = row < p.kv.rows ? paged_seq_of(qs, p.kv.n, row) : p.kv.n;
+    bool ok = seq < p.kv.n;
+    int pos = 0;
+    long long place = -1;
+    if (ok) {
+        pos = p.kv.kv_len[seq] - (qs[seq + 1] - row);
+        ok = pos >= 0 && (p.rot == 0 || pos < p.max_pos);
+        if (ok) place = paged_place(p.kv, seq, pos, 0);
+        ok = ok && place >= 0;
+    }
+    const bool turn = ok && 4 * c4 < p.rot;
+    PagedAngles angles;
+    angles.load(p, turn ? pos : 0, turn ? c4 : 0);     // (the tables' first row stands in)
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int row = row0 + u * RPB;
-        const int seq = row < p.kv.rows ? paged_seq_of(qs, p.kv.n, row) : p.kv.n;
-        bool ok = seq < p.kv.n;
-        int pos = 0;
-        long long place = -1;
-        if (ok) {
-            pos = p.kv.kv_len[seq] - (qs[seq + 1] - row);
-            ok = pos >= 0 && (p.rot == 0 || pos < p.max_pos);
-            if (ok) place = paged_place(p.kv, seq, pos, kind == 0 ? 0 : h);
-            ok = ok && place >= 0;
-        }
-        const f32x4 y = kind < 2 && p.rot ? paged_rope(p, x[u], pos, c4, ok) : x[u];
-        if (kind == 0) {
-            if (ok) *(f32x4*)(p.q_out + (long long)row * p.ldqo + h * HD + 4 * c4) = y;
+        const int head = blockIdx.y * U + u;
+        if (head >= all) continue;
+        const f32x4 y = head < p.heads + kh && p.rot ? paged_rope(p, x[u], angles, c4, turn) : x[u];
+        if (head < p.heads) {
+            if (ok) *(f32x4*)(p.q_out + at_row * p.ldqo + head * HD + 4 * c4) = y;
         } else {
-            paged_store<HD, TYPE>(kind == 1 ? p.kv.k : p.kv.v, kind == 1 ? p.kv.ks : p.kv.vs, place, y, c4, ok);
+            const bool is_k = head < p.heads + kh;
+            const int h = head - p.heads - (is_k ? 0 : kh);
+            paged_store<HD, TYPE>(is_k ? p.kv.k : p.kv.v, is_k ? p.kv.ks : p.kv.vs,
+                                  place + ((long long)h << p.kv.page_shift), y, c4, ok);
         }
     }
 }
 
 // ------------------------------------------------------------------ read
-// The inverse, in the same order: blockIdx.y the key heads, then the value
+// The inverse, in the same order: blockIdx.y over the key heads, then the value
 // heads.
 template <int HD, int TYPE, int U>
 __device__ __forceinline__ void kv_read(const KvReadParams& p) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR;
     __shared__ int qs[PAGED_MAX_SEQS + 1];
-    const int c4 = threadIdx.x % LPR, sub = threadIdx.x / LPR;
-    const bool is_v = (int)blockIdx.y >= p.kv.kv_heads;
-    const int h = is_v ? blockIdx.y - p.kv.kv_heads : blockIdx.y;
-    const void* pool = is_v ? p.kv.v : p.kv.k;
-    const float* scales = is_v ? p.kv.vs : p.kv.ks;
-    float* dst = is_v ? p.v_out : p.k_out;
-    const int row0 = blockIdx.x * (RPB * U) + sub;
+    const int c4 = threadIdx.x % LPR;
+    const int row = blockIdx.x * RPB + threadIdx.x / LPR;
+    const int kh = p.kv.kv_heads;
     paged_stage_starts(p.kv, qs);
-    long long place[U];
-    bool in[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int row = row0 + u * RPB;
-        const int seq = row < p.kv.rows ? paged_seq_of(qs, p.kv.n, row) : p.kv.n;
-        in[u] = seq < p.kv.n;
-        place[u] = in[u] ? paged_place(p.kv, seq, p.kv.kv_len[seq] - (qs[seq + 1] - row), h) : -1;
-    }
+    const int seq = row < p.kv.rows ? paged_seq_of(qs, p.kv.n, row) : p.kv.n;
+    if (seq >= p.kv.n) return;
+    const long long place = paged_place(p.kv, seq, p.kv.kv_len[seq] - (qs[seq + 1] - row), 0);
     f32x4 x[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
+        const int head = blockIdx.y * U + u < 2 * kh ? blockIdx.y * U + u : 2 * kh - 1;
+        const bool is_v = head >= kh;
+        const void* pool = is_v ? p.kv.v : p.kv.k;
         // row 0 of the pool stands in for a missing place, and is not used
-        const long long at = place[u] < 0 ? 0 : place[u];
+        const long long at = place < 0 ? 0 : place + ((long long)(is_v ? head - kh : head) << p.kv.page_shift);
         if (TYPE == KV_F32) {
             x[u] = *(const f32x4*)((const float*)pool + at * HD + 4 * c4);
         } else if (TYPE == KV_BF16) {
@@ -216,16 +231,17 @@ __device__ __forceinline__ void kv_read(const KvReadParams& p) {
                          __uint_as_float(w.y & 0xffff0000u)};
         } else {
             const int w = *(const int*)((const unsigned char*)pool + at * HD + 4 * c4);
-            const float s = scales[at];
+            const float s = (is_v ? p.kv.vs : p.kv.ks)[at];
             x[u] = f32x4{(float)(w << 24 >> 24) * s, (float)(w << 16 >> 24) * s, (float)(w << 8 >> 24) * s,
                          (float)(w >> 24) * s};
         }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int row = row0 + u * RPB;
-        if (in[u])
-            *(f32x4*)(dst + (long long)row * p.ld + h * HD + 4 * c4) = place[u] < 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : x[u];
+        const int head = blockIdx.y * U + u;
+        if (head >= 2 * kh) continue;
+        float* dst = head < kh ? p.k_out + (long long)row * p.ld + head * HD : p.v_out + (long long)row * p.ld + (head - kh) * HD;
+        *(f32x4*)(dst + 4 * c4) = place < 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : x[u];
     }
 }
 

@@ -18,7 +18,7 @@ struct TrlmServe {
     HipCtx* ctx;
     i32 device;
     /* looked up on first use of a head width and type */
-    hipFunction_t append[NHD][NTYPE][2], read[NHD][NTYPE][2], few[NHD][NTYPE], tile[NHD][NTYPE][2], join[NHD];
+    hipFunction_t append[NHD][NTYPE][2], read[NHD][NTYPE][2], few[NHD][NTYPE], tile[NHD][NTYPE], join[NHD][2];
     hipFunction_t rules[2][2];   /* [narrow, wide][aligned, not] */
 };
 
@@ -113,10 +113,11 @@ static PagedKv paged_kv(const TrlmKvCache* c, const TrlmKvSeqs* s) {
     return p;
 }
 
-/* Rows a 256-thread workgroup of the append and read kernels moves per head:
- * one per head_dim / 4 lanes, or four where that still leaves at least four
- * workgroups for each of the 256 compute units. */
-static int four_rows(u64 rows, u32 hd, u32 heads) { return cdiv64(rows, 4 * (1024 / hd)) * heads >= 1024; }
+/* A 256-thread workgroup of the append and read kernels moves 1024 / head_dim
+ * rows of one head, or of four heads where that still leaves at least four
+ * workgroups for each of the 256 compute units: the rows' places and angles are
+ * then found once for four heads. */
+static int four_heads(u64 rows, u32 hd, u32 heads) { return cdiv64(rows, 1024 / hd) * cdiv64(heads, 4) >= 1024; }
 
 i32 trlm_kv_append(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, const TrlmKvRows* r) {
     static const char* op = "trlm_kv_append";
@@ -150,10 +151,10 @@ i32 trlm_kv_append(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, cons
     p.max_pos = (int)r->max_pos; p.rot = (int)r->rot_dim; p.rot_half = r->rot_half != 0;
     const i32 i = hd_index(hd);
     const u32 heads = r->heads + 2 * c->kv_heads;
-    const int four = four_rows(s->rows, hd, heads);
+    const int four = four_heads(s->rows, hd, heads);
     void* args[] = { &p };
     hip_launch(kernel_hd(e, &e->append[i][c->type][four], four ? "k_kv_append4" : "k_kv_append", i, (i32)c->type),
-               (u32)cdiv64(s->rows, (four ? 4 : 1) * (1024 / hd)), heads, 1, 256, 1, 1, 0, args);
+               (u32)cdiv64(s->rows, 1024 / hd), (u32)cdiv64(heads, four ? 4 : 1), 1, 256, 1, 1, 0, args);
     return 0;
 }
 
@@ -174,10 +175,10 @@ i32 trlm_kv_read(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hipDev
     p.ld = (int)ld;
     const i32 i = hd_index(hd);
     const u32 heads = 2 * c->kv_heads;
-    const int four = four_rows(s->rows, hd, heads);
+    const int four = four_heads(s->rows, hd, heads);
     void* args[] = { &p };
     hip_launch(kernel_hd(e, &e->read[i][c->type][four], four ? "k_kv_read4" : "k_kv_read", i, (i32)c->type),
-               (u32)cdiv64(s->rows, (four ? 4 : 1) * (1024 / hd)), heads, 1, 256, 1, 1, 0, args);
+               (u32)cdiv64(s->rows, 1024 / hd), (u32)cdiv64(heads, four ? 4 : 1), 1, 256, 1, 1, 0, args);
     return 0;
 }
 
@@ -185,14 +186,27 @@ i32 trlm_kv_read(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hipDev
 
 #define FEW_TILE 16u      /* rows of a k_paged_attn_few workgroup */
 #define FEW_KEYS 128u     /* keys its four waves take at a time: splits are multiples of it */
-#define FEW_MAX 64u       /* rows (tokens x group) of a sequence up to which it is taken */
-#define TILE_KEYS 64u     /* keys of a k_paged_attn_tile stage */
-#define FEW_GROUPS 1024u  /* workgroups wanted: four for each of the 256 compute units */
-#define TILE_GROUPS 512u
+/* Workgroups of that kernel wanted.  Measured at 512 / 768 / 1024: 8 tokens over
+ * 16000 in bf16 69 / 57 / 72 us, 32 over 8192 in 8 bits 97 / 73 / 95, 64 over 1024
+ * in fp32 33.1 / 32.9 / 32.8. */
+#define FEW_GROUPS 768u
+/* A wave joins a row where the splits are more than 8, or the rows (tokens x
+ * heads) too few for a workgroup to take several: one token 9.6 us against 11.5,
+ * 1920 rows 13.9 against 15.7; 49152 rows of two splits 29 us against 9. */
+#define JOIN_SPLITS 8u
+#define JOIN_ROWS 16384u
+/* Rows (tokens x group) of a sequence up to which that kernel, which reads the
+ * keys once for every 16 rows, is the faster.  Measured, few against many rows'
+ * kernel: 24 sequences of 40 rows over 2000 tokens 15.8 / 34 us, 16 of 64 rows
+ * over 4000 70 / 147 us; of 128 rows 175 / 121 us. */
+#define FEW_MAX 64u
+#define TILE_ROWS 256u    /* rows of a k_paged_attn_tile workgroup: its registers fill a compute unit */
+#define TILE_KEYS 64u     /* keys of its stages */
+#define CUS 256u
 #define MAX_SPLITS 256u
 
 typedef struct AttnPlan {
-    u32 few_tiles, tiles, waves;      /* row tiles of a sequence in each kernel (0: not launched) */
+    u32 few_tiles, tiles;             /* row tiles of a sequence in each kernel (0: not launched) */
     u32 few_splits, tile_splits, chunk_few, chunk_tile, splits;
     u64 few_groups, tile_groups;
 } AttnPlan;
@@ -211,6 +225,42 @@ static u32 split_keys(u32 kv, u64 groups, u32 wanted, u32 unit, u32* chunk) {
     return (u32)cdiv64(kv, *chunk);
 }
 
+/* Splits for row tiles that take a compute unit each.  The time of s splits in
+ * keys: rounds of 256 workgroups, each as long as its keys and about 128 more
+ * for its start; the join about 64.  Where the new tokens are most of the
+ * context the workgroups have all lengths up to a split's and are taken longest
+ * first, so that the units share the sum.  Otherwise sequences that are shorter
+ * than the longest leave units idle in large splits: among several sequences the
+ * most splits within a tenth of the least time are taken.  (Measured, splits and
+ * us: 8 x 1024 prompts 2 50.8, 4 56.5; 2048 tokens over 16384 1 1120, 2 1154,
+ * 4 1198; 512 over 8192 16 46.1, 32 59.7; 4096 from empty 1 390, 2 296, 4 349;
+ * 16 ragged sequences of 32 over 4000 2 170, 4 121.) */
+static u32 split_tiles(u32 kv, u32 max_q, u64 groups, u32 n, u32* chunk) {
+    u64 best = 0;
+    u32 best_s = 1;
+    *chunk = (u32)(cdiv64(kv, TILE_KEYS) * TILE_KEYS);
+    for (u32 s = 1; s <= MAX_SPLITS && (s == 1 || s * groups <= 4 * CUS); s++) {
+        const u32 c = (u32)(cdiv64(cdiv64(kv, s), TILE_KEYS) * TILE_KEYS);
+        if (cdiv64(kv, c) != s) continue;
+        const u64 wgs = groups * s;
+        const int uniform = 2ull * max_q < kv;
+        u64 t;
+        if (uniform) {
+            t = cdiv64(wgs, CUS) * (c + 128);
+        } else {
+            const u64 share = wgs * c / CUS * (2ull * kv - max_q) / (2ull * kv);
+            t = (share > c ? share : c) + 128 * cdiv64(wgs, CUS);
+        }
+        t += s > 1 ? 64 : 0;
+        if (!best || t < best || (uniform && n > 1 && 10 * t <= 11 * best)) {
+            if (!best || t < best) best = t;
+            best_s = s;
+            *chunk = c;
+        }
+    }
+    return best_s;
+}
+
 /* A call's launch shape, from what the host knows of it alone, so that a
  * captured call keeps it. */
 static AttnPlan attn_plan(const TrlmKvCache* c, const TrlmKvSeqs* s, u32 heads) {
@@ -223,16 +273,14 @@ static AttnPlan attn_plan(const TrlmKvCache* c, const TrlmKvSeqs* s, u32 heads) 
     p.few_groups = seq_heads * p.few_tiles;
     p.few_splits = split_keys(kv, p.few_groups, FEW_GROUPS, FEW_KEYS, &p.chunk_few);
     p.chunk_tile = p.chunk_few;
-    p.splits = p.few_splits;
     if (most > FEW_MAX) {
-        p.waves = seq_heads * cdiv64(most, 256) >= 256 ? 8 : 4;
-        p.tiles = (u32)cdiv64(most, 32 * p.waves);
+        p.tiles = (u32)cdiv64(most, TILE_ROWS);
         p.tile_groups = seq_heads * p.tiles;
-        p.tile_splits = split_keys(kv, p.tile_groups, TILE_GROUPS, TILE_KEYS * 4, &p.chunk_tile);
-        if (p.tile_splits > p.splits) p.splits = p.tile_splits;
+        p.tile_splits = split_tiles(kv, max_q, p.tile_groups, s->n, &p.chunk_tile);
         /* one sequence, or as many rows as all sequences at their longest: none is short */
         if (s->n == 1 || (u64)s->n * max_q <= s->rows) p.few_splits = 0;
     }
+    p.splits = p.tile_splits > p.few_splits ? p.tile_splits : p.few_splits;
     return p;
 }
 
@@ -260,7 +308,7 @@ i32 trlm_attn_paged(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hip
     const AttnPlan pl = attn_plan(c, s, heads);
     const u64 need = attn_ws(c, s, heads, &pl);
     if (need && (unaligned(ws, 16) || ws_bytes < need)) return refuse(op, "the workspace is too small or not 16-byte aligned");
-    if (pl.few_groups > 0x7fffffffull || pl.tile_groups > 0x7fffffffull || cdiv64((u64)s->rows * heads, 1024 / hd) > 0x7fffffffull)
+    if (pl.few_groups > 0x7fffffffull || pl.tile_groups > 0x7fffffffull || (u64)s->rows * heads > 0x7fffffffull)
         return refuse(op, "too many workgroups");
     PagedAttnParams p;
     memset(&p, 0, sizeof(p));
@@ -277,24 +325,29 @@ i32 trlm_attn_paged(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hip
     const i32 i = hd_index(hd);
     void* args[] = { &p };
     if (pl.tiles)
-        hip_launch(kernel_hd(e, &e->tile[i][c->type][pl.waves == 8], pl.waves == 8 ? "k_paged_attn_tile8" :
-                             "k_paged_attn_tile4", i, (i32)c->type), (u32)pl.tile_groups, pl.tile_splits, 1,
-                   64 * pl.waves, 1, 1, 0, args);
+        hip_launch(kernel_hd(e, &e->tile[i][c->type], "k_paged_attn_tile", i, (i32)c->type), (u32)pl.tile_groups,
+                   pl.tile_splits, 1, 512, 1, 1, 0, args);
     if (pl.few_splits)
         hip_launch(kernel_hd(e, &e->few[i][c->type], "k_paged_attn_few", i, (i32)c->type), (u32)pl.few_groups,
                    pl.few_splits, 1, 256, 1, 1, 0, args);
-    if (pl.splits > 1)
-        hip_launch(kernel_hd(e, &e->join[i], "k_paged_attn_join", i, -1),
-                   (u32)cdiv64((u64)s->rows * heads, 1024 / hd), 1, 1, 256, 1, 1, 0, args);
+    if (pl.splits > 1) {
+        const int many = pl.splits > JOIN_SPLITS || (u64)s->rows * heads < JOIN_ROWS;
+        hip_launch(kernel_hd(e, &e->join[i][many], many ? "k_paged_attn_join_long" : "k_paged_attn_join", i, -1),
+                   (u32)cdiv64((u64)s->rows * heads, many ? 4 : 1024 / hd), 1, 1, 256, 1, 1, 0, args);
+    }
     return 0;
 }
 
 /* ---------------- rules on logits ---------------- */
 
-/* Tokens a workgroup takes of its row: 4096, or 1024 where that leaves fewer
- * than two workgroups for each of the 256 compute units. */
+/* Tokens a workgroup takes of its row: 1024; or 4096, so that a history is read
+ * by fewer of them, where that leaves 16 workgroups for each of the 256 compute
+ * units.  Measured, wide against narrow: 64 rows of 31769 tokens and 1024 of
+ * history 7.7 / 6.6 us, 64 of 131072 and 2048 16.8 / 15.9, 256 of them 56.5 / 61.1;
+ * without a history 50.9 / 46.2. */
 #define RULES_WIDE 4096u
 #define RULES_NARROW 1024u
+#define RULES_WIDE_MIN 4096u
 
 i32 trlm_logits_rules(TrlmServe* e, const TrlmLogitsRules* r) {
     static const char* op = "trlm_logits_rules";
@@ -325,7 +378,7 @@ i32 trlm_logits_rules(TrlmServe* e, const TrlmLogitsRules* r) {
     p.ld = r->ld; p.ld_out = r->ld_out; p.ld_hist = r->ld_hist; p.ld_bias = r->ld_bias; p.ld_mask = r->ld_mask;
     p.vocab = (int)r->vocab;
     const int u = unaligned(r->logits, 16) || unaligned(r->out, 16) || (r->ld | r->ld_out) % 4;
-    const int wide = cdiv64(r->vocab, RULES_WIDE) * r->rows >= 512;
+    const int wide = r->history && cdiv64(r->vocab, RULES_WIDE) * r->rows >= RULES_WIDE_MIN;
     static const char* const NAMES[2][2] = { { "k_logits_rules_1024", "k_logits_rules_1024_u" },
                                              { "k_logits_rules_4096", "k_logits_rules_4096_u" } };
     void* args[] = { &p };

@@ -190,6 +190,10 @@ i32 trlm_kv_read(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hipDev
  * 16000 in bf16 69 / 57 / 72 us, 32 over 8192 in 8 bits 97 / 73 / 95, 64 over 1024
  * in fp32 33.1 / 32.9 / 32.8. */
 #define FEW_GROUPS 768u
+/* Contexts up to which one workgroup takes all keys, two turns of its waves, and
+ * saves the join: one token over 200 7.7 us against 9.3; over 500 12.4 against
+ * 10.6. */
+#define FEW_WHOLE 256u
 /* A wave joins a row where the splits are more than 8, or the rows (tokens x
  * heads) too few for a workgroup to take several: one token 9.6 us against 11.5,
  * 1920 rows 13.9 against 15.7; 49152 rows of two splits 29 us against 9. */
@@ -272,6 +276,10 @@ static AttnPlan attn_plan(const TrlmKvCache* c, const TrlmKvSeqs* s, u32 heads) 
     p.few_tiles = (u32)cdiv64(most < FEW_MAX ? most : FEW_MAX, FEW_TILE);
     p.few_groups = seq_heads * p.few_tiles;
     p.few_splits = split_keys(kv, p.few_groups, FEW_GROUPS, FEW_KEYS, &p.chunk_few);
+    if (kv <= FEW_WHOLE) {
+        p.few_splits = 1;
+        p.chunk_few = (u32)(cdiv64(kv, FEW_KEYS) * FEW_KEYS);
+    }
     p.chunk_tile = p.chunk_few;
     if (most > FEW_MAX) {
         p.tiles = (u32)cdiv64(most, TILE_ROWS);

@@ -142,6 +142,46 @@ typedef struct TrlmLogitsRules {
 
 i32 trlm_logits_rules(TrlmServe* e, const TrlmLogitsRules* r);
 
+/* ---- decoding many sequences of their own lengths ----
+ * A decoder over the trainer's resident parameters, on its stream, with one
+ * paged cache a layer.  Sequences are slots 0 .. max_seqs - 1; a slot is empty
+ * until gpu_paged_extend gives it tokens and again after gpu_paged_release.
+ * head_dim is one of the operators'; num_pages x page_size at most 2^36.
+ * Where a call returns i32: 0, or -1 with a message on stderr and nothing
+ * changed (a slot, token or length out of range, a slot twice in a call, no
+ * pages left).  Creation with sizes out of range ends the process, as the
+ * trainer's does. */
+typedef struct TrlmPagedDecoder TrlmPagedDecoder;
+TrlmPagedDecoder* gpu_paged_create(GpuTrainer* g, u32 max_seqs, u32 max_ctx, u32 num_pages, u32 page_size, u32 kv_type);
+void gpu_paged_destroy(TrlmPagedDecoder* d);
+/* lens[i] new tokens (at least one) of slot seqs[i], i < n, their ids one after
+ * the other: prompts, chunks of them and single tokens in one call.  Leaves the
+ * logits of every slot's last token as rows 0 .. n - 1. */
+i32 gpu_paged_extend(TrlmPagedDecoder* d, u32 n, const u32* seqs, const u32* lens, const u32* ids);
+void gpu_paged_release(TrlmPagedDecoder* d, u32 seq);
+u32 gpu_paged_length(const TrlmPagedDecoder* d, u32 seq);   /* 0 for an empty slot or none */
+u32 gpu_paged_free_pages(const TrlmPagedDecoder* d);
+/* On the rows of the last extend: the logits [n][V]; rules on them (a slot's
+ * history is its tokens, those after its first extend count as generated, a released
+ * slot has none; each
+ * pointer may be NULL; host arrays of n entries or rows); the first maximum of
+ * each row (0 where a mask left nothing); sample_next (generate.c:57-73) per
+ * row, as gpu_decoder_sample (the last token where a mask left nothing). */
+typedef struct TrlmTokenRules {
+    const f32 *repetition, *frequency, *presence;   /* [n] */
+    const u32* bias_ids;                            /* [n][ld_bias] */
+    const f32* bias;                                /* [n][ld_bias] */
+    const u32* n_bias;                              /* [n], up to ld_bias */
+    u32 ld_bias;
+    const u32* mask;                                /* [n][ceil(V / 32)] */
+} TrlmTokenRules;
+void gpu_paged_logits(TrlmPagedDecoder* d, f32* host_logits);
+i32 gpu_paged_rules(TrlmPagedDecoder* d, const TrlmTokenRules* r);
+void gpu_paged_greedy(TrlmPagedDecoder* d, u32* out_ids);
+void gpu_paged_sample(TrlmPagedDecoder* d, PCGState* rngs, f32 temperature, u32* out_ids);
+/* The cached rows of a slot in one layer, k and v [length][d_model]. */
+i32 gpu_paged_read(TrlmPagedDecoder* d, u32 seq, u32 layer, f32* k, f32* v);
+
 #ifdef __cplusplus
 }
 #endif

@@ -164,7 +164,11 @@ def test_other_arguments_out_of_range(host, trlm, capfd):
     c, s = cache(trlm), seqs(trlm)
     for a in ((None, 0x2000, 128), (0x1000, None, 128), (0x1004, 0x2000, 128), (0x1000, 0x2000, 126), (0x1000, 0x2000, 124)):
         refused(host, lambda: host.trlm_kv_read(host.e, c, s, *a), capfd, "trlm_kv_read")
+    assert host.trlm_attn_paged_workspace(c, s, 4) == 0  # a short context is not split: no workspace is asked for
+    taken(host, lambda: host.trlm_attn_paged(host.e, c, s, 0x1000, 512, 4, 0.125, 0x2000, 512, None, 0), capfd)
+    s = seqs(trlm, max_pages=40, max_kv=2000)
     ws = host.trlm_attn_paged_workspace(c, s, 4)
+    assert ws > 0
     good = (0x1000, 512, 4, 0.125, 0x2000, 512, 0x3000, ws)
     taken(host, lambda: host.trlm_attn_paged(host.e, c, s, *good), capfd)
     for at, v in ((0, None), (0, 0x1004), (1, 252), (1, 510), (2, 0), (2, 3), (2, 1026), (4, None), (5, 252), (6, 0x3008),
@@ -239,15 +243,16 @@ def test_header_and_binding_agree(trlm, tmp_path):
     with open(os.path.join(ROOT, "include", "trlm_serve.h")) as fh:
         text = re.sub(r"/\*.*?\*/", "", fh.read(), flags=re.S)
     _, hip = trlm.libs()
-    names = set(re.findall(r"^(?:i32|u32|u64|f32|void|TrlmServe\*|const char\*|[A-Z]\w+\*) ((?:trlm|gpu)_\w+)\(", text, re.M))
-    assert {"trlm_serve_create", "trlm_serve_destroy", "trlm_kv_append", "trlm_kv_read", "trlm_attn_paged",
-            "trlm_attn_paged_workspace", "trlm_logits_rules"} <= names
+    names = set(re.findall(r"^(?:i32|u32|u64|f32|void|[A-Z]\w+\*) ((?:trlm|gpu)_\w+)\(", text, re.M))
+    assert {"gpu_paged_create", "gpu_paged_extend", "gpu_paged_rules", "gpu_paged_read", "trlm_serve_create",
+            "trlm_serve_destroy", "trlm_kv_append", "trlm_kv_read", "trlm_attn_paged", "trlm_attn_paged_workspace",
+            "trlm_logits_rules"} <= names
     for n in names:
         assert hasattr(hip, n), n
     if not os.path.exists(os.path.join(ROCM_INC, "hip", "hip_runtime_api.h")):
         return
     mirrors = {"TrlmKvCache": trlm.KvCache, "TrlmKvSeqs": trlm.KvSeqs, "TrlmKvRows": trlm.KvRows,
-               "TrlmLogitsRules": trlm.LogitsRules}
+               "TrlmLogitsRules": trlm.LogitsRules, "TrlmTokenRules": trlm.TokenRules}
     out = []
     for s, m in mirrors.items():
         out += ['printf("%%zu ", sizeof(%s));' % s] + ['printf("%%zu ", offsetof(%s, %s));' % (s, f) for f, _ in m._fields_]

@@ -4,7 +4,7 @@ Outputs (next to this file, git-ignored, shipped to the GPU box as built):
   trlm_kernels.hsaco  gfx950 code object with every kernel (hipcc --genco)
   libtrlm_hip.so      the drop-in C library: hip_backend.c, trlm_gemm.c,
                       gpu_train.c, gpu_decode.c, checkpoint.c, train_loop.c,
-                      gpu_ops.c, serve.c (gcc, HIP runtime API)
+                      gpu_ops.c, serve.c, gpu_paged.c (gcc, HIP runtime API)
   libtrlm_host.so     standalone host runtime (allocator, tensors, nodes,
                       PCG, scalar maths, RoPE tables) for use without the
                       reference's own runtime objects
@@ -48,7 +48,7 @@ def build_host():
 
 def build_hip_lib():
     srcs = [os.path.join(CSRC, f) for f in ("hip_backend.c", "trlm_gemm.c", "gpu_train.c", "gpu_decode.c", "checkpoint.c",
-                                            "train_loop.c", "gpu_ops.c", "serve.c")]
+                                            "train_loop.c", "gpu_ops.c", "serve.c", "gpu_paged.c")]
     # noalloc.hip holds the no-allocation GEMM's scratch array (a __device__
     # global of this library, not of the kernel image) and its entry point.
     _run([os.path.join(ROCM, "bin", "hipcc"), "-c", "-fPIC", "--offload-arch=gfx950", "-O3", "-Xclang",

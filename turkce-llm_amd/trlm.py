@@ -130,6 +130,13 @@ class LogitsRules(C.Structure):
                 ("ld_mask", C.c_uint32)]
 
 
+class TokenRules(C.Structure):
+    """Mirror of TrlmTokenRules: rules on the rows of a paged decoder."""
+    _fields_ = [("repetition", C.c_void_p), ("frequency", C.c_void_p), ("presence", C.c_void_p),
+                ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("n_bias", C.c_void_p), ("ld_bias", C.c_uint32),
+                ("mask", C.c_void_p)]
+
+
 _libs = None
 
 
@@ -284,6 +291,17 @@ def _bind(host, hip):
     _sig(hip, "trlm_attn_paged", C.c_int32, [C.c_void_p, cache, seqs, C.c_void_p, C.c_uint32, C.c_uint32, C.c_float,
                                              C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint64])
     _sig(hip, "trlm_logits_rules", C.c_int32, [C.c_void_p, C.POINTER(LogitsRules)])
+    _sig(hip, "gpu_paged_create", DP, [GP] + [C.c_uint32] * 5)
+    _sig(hip, "gpu_paged_destroy", None, [DP])
+    _sig(hip, "gpu_paged_extend", C.c_int32, [DP, C.c_uint32, u32p, u32p, u32p])
+    _sig(hip, "gpu_paged_release", None, [DP, C.c_uint32])
+    _sig(hip, "gpu_paged_length", C.c_uint32, [DP, C.c_uint32])
+    _sig(hip, "gpu_paged_free_pages", C.c_uint32, [DP])
+    _sig(hip, "gpu_paged_logits", None, [DP, f32p])
+    _sig(hip, "gpu_paged_rules", C.c_int32, [DP, C.POINTER(TokenRules)])
+    _sig(hip, "gpu_paged_greedy", None, [DP, u32p])
+    _sig(hip, "gpu_paged_sample", None, [DP, C.POINTER(PCGState), C.c_float, u32p])
+    _sig(hip, "gpu_paged_read", C.c_int32, [DP, C.c_uint32, C.c_uint32, f32p, f32p])
     _sig(hip, "gpu_ops_pin", None, [C.c_void_p, C.c_uint64])
     _sig(hip, "gpu_ops_unpin_all", None, [])
 
@@ -680,3 +698,73 @@ class Serve:
     def close(self):
         self.hip.trlm_serve_destroy(self.e)
         self.e = None
+
+
+class PagedDecoder:
+    """gpu_paged_* over a Trainer's resident parameters: sequences of their
+    own lengths over one paged cache."""
+
+    def __init__(self, trainer, max_seqs, max_ctx, num_pages, page_size=64, kv_type=KV_F32):
+        self.hip, self.tr, self.V, self.D = trainer.hip, trainer, trainer.hm.V, trainer.hm.D
+        self.d = self.hip.gpu_paged_create(C.byref(trainer.g), max_seqs, max_ctx, num_pages, page_size, kv_type)
+        self.n = 0
+
+    def extend(self, seqs, tokens):
+        """tokens: one array of new ids for each slot of seqs."""
+        tokens = [_u32(t).ravel() for t in tokens]
+        if len(seqs) != len(tokens):
+            raise ValueError("%d slots, tokens for %d" % (len(seqs), len(tokens)))
+        lens = _u32([t.size for t in tokens])
+        ids = np.concatenate(tokens) if tokens else np.zeros(0, np.uint32)
+        Serve._checked(self.hip.gpu_paged_extend(self.d, len(tokens), _u32(seqs), lens, ids), "gpu_paged_extend")
+        self.n = len(tokens)
+
+    def release(self, seq):
+        self.hip.gpu_paged_release(self.d, seq)
+
+    def length(self, seq):
+        return self.hip.gpu_paged_length(self.d, seq)
+
+    def free_pages(self):
+        return self.hip.gpu_paged_free_pages(self.d)
+
+    def logits(self):
+        out = np.zeros((self.n, self.V), np.float32)
+        self.hip.gpu_paged_logits(self.d, out)
+        return out
+
+    def rules(self, repetition=None, frequency=None, presence=None, bias_ids=None, bias=None, n_bias=None, mask=None):
+        a = [None if x is None else np.ascontiguousarray(x, t) for x, t in (
+            (repetition, np.float32), (frequency, np.float32), (presence, np.float32), (bias_ids, np.uint32),
+            (bias, np.float32), (n_bias, np.uint32), (mask, np.uint32))]
+        width = 0 if a[3] is None else a[3].shape[-1]
+        for x, tail in zip(a, ((), (), (), (width,), (width,), (), ((self.V + 31) // 32,))):
+            if x is not None and x.shape != (self.n,) + tail:
+                raise ValueError("rules of shape %r for %d rows" % (x.shape, self.n))
+        p = [None if x is None else x.ctypes.data for x in a]
+        r = TokenRules(*p[:6], width, p[6])
+        Serve._checked(self.hip.gpu_paged_rules(self.d, C.byref(r)), "gpu_paged_rules")
+
+    def greedy(self):
+        out = np.zeros(self.n, np.uint32)
+        self.hip.gpu_paged_greedy(self.d, out)
+        return out
+
+    def sample(self, rngs, temperature):
+        """rngs: ctypes array of PCGState (one per row), advanced in place."""
+        if len(rngs) < self.n:
+            raise ValueError("%d generators for %d rows" % (len(rngs), self.n))
+        out = np.zeros(self.n, np.uint32)
+        self.hip.gpu_paged_sample(self.d, rngs, temperature, out)
+        return out
+
+    def read(self, seq, layer):
+        n = self.length(seq)
+        k, v = np.zeros((n, self.D), np.float32), np.zeros((n, self.D), np.float32)
+        Serve._checked(self.hip.gpu_paged_read(self.d, seq, layer, k, v), "gpu_paged_read")
+        return k, v
+
+    def destroy(self):
+        if self.d is not None:
+            self.hip.gpu_paged_destroy(self.d)
+            self.d = None

@@ -102,8 +102,8 @@ i32 trlm_kv_read(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hipDev
 
 /* out row r, head h = sum over the tokens t <= position of r of softmax(scale
  * <q_r, k_t>) v_t, query head h reading cached head h / (heads / kv_heads).
- * q and out: fp32 rows, heads side by side, strides in floats; out may not
- * overlap q.  Accuracy as of fp32 products and sums, for every cache type.  A
+ * q and out: fp32 rows (rows * heads below 2^31), heads side by side, strides
+ * in floats; out may not overlap q.  Accuracy as of fp32 products and sums, for every cache type.  A
  * row without tokens to see (kv_len 0, no pages) is zeros.  A number that is
  * not finite makes the outputs that see it NaN (an infinite key whose score
  * is -infinity may also count as if it were not there) and no others: tokens after a row's

@@ -600,3 +600,166 @@ def test_captured_calls_follow_their_buffers(trlm, box):
     finally:
         hip.hipGraphExecDestroy(exe)
         hip.hipGraphDestroy(graph)
+
+
+# ---------------------------------------------------------------- calls at the edges of what is allowed
+
+@pytest.mark.parametrize("type", ALL_TYPES)
+@pytest.mark.parametrize("q_len,kv_len,spare,max_q", [([10], [40], 90, 100), ([1], [700], 299, 300), ([0], [9], 64, 64),
+                                                      ([10, 3], [500, 3], 187, 100), ([1, 100], [1, 100], 99, 100),
+                                                      ([3, 70], [900, 900], 0, 400)])
+def test_attn_bounds_wider_than_the_call(trlm, box, type, q_len, kv_len, spare, max_q):
+    """max_q and rows are bounds: a call that could hold long chunks and holds short ones."""
+    attn_case(trlm, box, np.random.default_rng(47), type, 64, 4, 2, q_len, kv_len, 32, spare_rows=spare, max_q=max_q)
+
+
+@pytest.mark.parametrize("type", ALL_TYPES)
+@pytest.mark.parametrize("page", [16, 65536])
+def test_page_sizes_at_the_ends(trlm, box, type, page):
+    rng = np.random.default_rng(53)
+    attn_case(trlm, box, rng, type, 16, 2, 1, [1, 90, 7], [17, 90, 1500], page)
+    append_case(trlm, box, rng, type, 16, 2, 1, [1, 90, 7], [17, 90, 1500], page, 16, False)
+
+
+@pytest.mark.parametrize("type", ALL_TYPES)
+def test_starts_out_of_range_are_kept_to_the_rows(trlm, box, type):
+    """Row ranges that break the rules (negative, descending, past the end): nothing outside the buffers is touched."""
+    dev, serve = box
+    dev.current()
+    rng = np.random.default_rng(59)
+    H, Hkv, hd, page, rows, guard = 4, 2, 64, 16, 90, 40
+    ld = (H + 2 * Hkv) * hd
+    for starts in ([-5, 3, 2, 1000, 80], [50, 20, 90, 2 ** 31 - 1, -2 ** 31], [-2 ** 31, -1, 0, 40, 2 ** 31 - 1]):
+        for max_q in (4, 90):
+            seqs = ref.Seqs(rng, [20] * 4, [33] * 4, page)
+            shape = (seqs.num, Hkv, page, hd)
+            pool = ref.Pool(type, seqs.num, page, Hkv, hd, rng.standard_normal(shape).astype(np.float32),
+                            rng.standard_normal(shape).astype(np.float32))
+            seqs.q_start, seqs.rows, seqs.max_q, seqs.max_kv = np.array(starts, np.int32), rows, max_q, 3000
+            seqs.kv_len = [33, 2 ** 31 - 1, -2 ** 31, 5]
+            cache, s = pool.upload(dev, trlm), seqs.upload(dev, trlm)
+            cos, sin = tables(64, hd)
+            whole = rng.standard_normal((rows + 2 * guard, ld)).astype(np.float32)
+            d_x, d_cos, d_sin = dev.upload(whole), dev.upload(cos), dev.upload(sin)
+            x = d_x + 4 * guard * ld
+            d_o, d_k, d_v = [dev.upload(whole) for _ in range(3)]
+            rows_ = trlm.KvRows(q=x, k=x + 4 * H * hd, v=x + 4 * (H + Hkv) * hd, ldq=ld, ldk=ld, ldv=ld, q_out=x, ldqo=ld,
+                                heads=H, cos_t=d_cos, sin_t=d_sin, max_pos=64, rot_dim=hd, rot_half=0)
+            ws_bytes = serve.attn_workspace(cache, s, H)
+            edge = np.full(1024, 3.0, np.float32)
+            d_ws = dev.upload(np.concatenate([edge, np.zeros(ws_bytes // 4, np.float32), edge]))
+            serve.append(cache, s, rows_)
+            serve.attn(cache, s, x, ld, H, 0.125, d_o + 4 * guard * ld, ld, d_ws + 4096, ws_bytes)
+            serve.read(cache, s, d_k + 4 * guard * ld, d_v + 4 * guard * ld, ld)
+            for p in (d_x, d_o, d_k, d_v):
+                got = dev.download(p, whole.shape)
+                assert np.array_equal(got[:guard], whole[:guard]) and np.array_equal(got[-guard:], whole[-guard:])
+            got = dev.download(d_ws, (2048 + ws_bytes // 4,))
+            assert np.array_equal(got[:1024], edge) and np.array_equal(got[-1024:], edge)
+            for p in pool.ptr + seqs.ptr + [d_x, d_o, d_k, d_v, d_cos, d_sin, d_ws]:
+                if p:
+                    dev.free(p)
+
+
+@pytest.mark.parametrize("type,numbers", [("f32", 2 ** 32), ("bf16", 2 ** 32), ("i8", 5 * 2 ** 30)])
+def test_offsets_past_32_bits(trlm, box, type, numbers):
+    """A pool of more than 2^32 numbers, the pages in use at both of its ends; rows 2^30 floats apart."""
+    dev, serve = box
+    dev.current()
+    rng = np.random.default_rng(61)
+    H, Hkv, hd, page = 2, 2, 64, 64
+    num = numbers // (Hkv * page * hd) + 3
+    small = ref.Seqs(rng, [100, 1], [100, 1], page)
+    small.pages = np.array([[0, 1], [2, 3]], np.int32)
+    pool = ref.Pool(type, 4, page, Hkv, hd)
+    size = {"f32": 4, "bf16": 2, "i8": 1}[type]
+    d = {n: dev.hip.hip_alloc(num * Hkv * page * hd * size) for n in "kv"}
+    sc = {n: dev.hip.hip_alloc(num * Hkv * page * 4) for n in "kv"} if type == "i8" else dict(k=None, v=None)
+    cache = trlm.KvCache(k=d["k"], v=d["v"], k_scale=sc["k"], v_scale=sc["v"], type=ref.TYPES[type], num_pages=num,
+                         page_size=page, kv_heads=Hkv, head_dim=hd)
+    far = small.pages.copy()
+    small.pages = np.array([[num - 1, 0], [num - 3, num - 2]], np.int32)
+    s = small.upload(dev, trlm)
+    small.pages = far
+    ld = 3 * H * hd
+    x = rng.standard_normal((101, ld)).astype(np.float32)
+    d_x = dev.upload(x)
+    serve.append(cache, s, trlm.KvRows(q=None, k=d_x + 4 * H * hd, v=d_x + 8 * H * hd, ldq=0, ldk=ld, ldv=ld, q_out=None,
+                                       ldqo=0, heads=0, cos_t=None, sin_t=None, max_pos=0, rot_dim=0, rot_half=0))
+    for r in range(101):
+        pg, at = small.pages[0 if r < 100 else 1][r % 100 // page], r % 100 % page
+        for j, n in enumerate("kv"):
+            stored, scale = pool.store(x[r, (1 + j) * H * hd:(2 + j) * H * hd].reshape(Hkv, hd))
+            getattr(pool, n)[pg, :, at] = stored
+            if scale is not None:
+                getattr(pool, n + "s")[pg, :, at] = scale
+    outs = [dev.empty(4 * 101 * Hkv * hd) for _ in "kv"]
+    serve.read(cache, s, outs[0], outs[1], Hkv * hd)
+    for n, o in zip("kv", outs):
+        got = dev.download(o, (101, Hkv, hd))
+        for r in range(101):
+            pg, at = small.pages[0 if r < 100 else 1][r % 100 // page], r % 100 % page
+            assert np.array_equal(got[r], pool.numbers(n)[pg, :, at].astype(np.float32))
+    want, bound = ref.attention(pool, small, x, H, 0.125)
+    ws_bytes = serve.attn_workspace(cache, s, H)
+    ws, d_o = dev.empty(ws_bytes), dev.empty(4 * 101 * H * hd)
+    serve.attn(cache, s, d_x, ld, H, 0.125, d_o, H * hd, ws, ws_bytes)
+    assert np.all(np.abs(dev.download(d_o, (101, H, hd)) - want) <= bound[..., None])
+    if type == "bf16":
+        # the second sequence's token and two more rows, 2^30 floats apart (row 2 is 2^31 floats and 2^33 bytes in)
+        wide = ref.Seqs(rng, [2, 1], [100, 1], page)
+        wide.pages = np.array([[num - 1, 0], [num - 3, num - 2]], np.int32)
+        s2 = wide.upload(dev, trlm)
+        gap = 2 ** 30
+        d_q, d_w = [dev.hip.hip_alloc(4 * (2 * gap + H * hd)) for _ in "qo"]
+        y = x[98:]
+        for r in range(3):
+            row = np.ascontiguousarray(y[r, :H * hd])
+            dev.hip.hip_h2d(d_q + 4 * r * gap, row.ctypes.data, row.nbytes)
+        ws2 = dev.empty(serve.attn_workspace(cache, s2, H))
+        serve.attn(cache, s2, d_q, gap, H, 0.125, d_w, gap, ws2, serve.attn_workspace(cache, s2, H))
+        for r in range(3):
+            got = dev.download(d_w + 4 * r * gap, (H, hd))
+            assert np.all(np.abs(got - want[98 + r]) <= bound[98 + r][:, None])
+        rule = trlm.LogitsRules(logits=d_q, out=d_w, rows=3, vocab=H * hd, ld=gap, ld_out=gap)
+        serve.logits_rules(rule)
+        for r in range(3):
+            assert np.array_equal(dev.download(d_w + 4 * r * gap, (H * hd,)), y[r, :H * hd])
+        for p in [d_q, d_w, ws2] + wide.ptr:
+            dev.free(p)
+    for p in list(d.values()) + [p for p in sc.values() if p] + outs + [d_x, ws, d_o] + small.ptr:
+        dev.free(p)
+
+
+def test_two_contexts_at_once(trlm, box):
+    """Two contexts, each with its own stream, handle and workspace, their calls queued in turn before either is waited
+    for: the same as alone."""
+    dev, serve = box
+    dev2 = trlm.Device()
+    serve2 = trlm.Serve(dev2)
+    rng = np.random.default_rng(67)
+    H, Hkv, hd, page = 4, 2, 64, 32
+    jobs = []
+    for d, e in ((dev, serve), (dev2, serve2)):
+        d.current()
+        seqs = ref.Seqs(rng, [1, 200, 3], [900, 400, 3], page)
+        shape = (seqs.num, Hkv, page, hd)
+        pool = ref.Pool("bf16", seqs.num, page, Hkv, hd, rng.standard_normal(shape).astype(np.float32),
+                        rng.standard_normal(shape).astype(np.float32))
+        q = rng.standard_normal((seqs.rows, H * hd)).astype(np.float32)
+        cache, s = pool.upload(d, trlm), seqs.upload(d, trlm)
+        n = e.attn_workspace(cache, s, H)
+        jobs.append((d, e, cache, s, d.upload(q), d.empty(q.nbytes), d.empty(n), n, ref.attention(pool, seqs, q, H, 0.125),
+                     q.shape))
+    for _ in range(20):
+        for d, e, cache, s, q, o, ws, n, _, _ in jobs:
+            d.current()
+            e.attn(cache, s, q, H * hd, H, 0.125, o, H * hd, ws, n)
+    for d, e, cache, s, q, o, ws, n, (want, bound), shape in jobs:
+        d.current()
+        got = d.download(o, shape).reshape(-1, H, hd)
+        assert np.all(np.abs(got - want) <= bound[..., None])
+    dev2.current()
+    serve2.close()
+    dev2.close()
+    dev.current()

@@ -176,6 +176,20 @@ def test_other_arguments_out_of_range(host, trlm, capfd):
         a = list(good)
         a[at] = v
         refused(host, lambda: host.trlm_attn_paged(host.e, c, s, *a), capfd, "trlm_attn_paged")
+    s = seqs(trlm, rows=2 ** 21, max_q=1, max_kv=64)
+    c = cache(trlm, kv_heads=1, head_dim=16)
+    refused(host, lambda: host.trlm_attn_paged(host.e, c, s, 0x1000, 16384, 1024, 0.125, 0x2000, 16384, 0x3000, 2 ** 62),
+            capfd, "trlm_attn_paged")
+    # more threads than a launch holds: 2^24 workgroups of 256, 2^23 of 512, 2^24 of joins
+    c = cache(trlm, kv_heads=1024, head_dim=16, num_pages=1000)
+    for heads, k in ((1024, dict(n=4096, rows=4096 * 64, max_q=64)), (1024, dict(n=2048, rows=2 ** 20, max_q=1024))):
+        s = seqs(trlm, max_kv=64, **k)
+        refused(host, lambda: host.trlm_attn_paged(host.e, c, s, 0x1000, 16384, heads, 0.125, 0x2000, 16384, 0x3000, 2 ** 62),
+                capfd, "trlm_attn_paged")
+    c, s = cache(trlm, kv_heads=1, head_dim=128), seqs(trlm, n=1, rows=2 ** 20, max_q=1, max_kv=2 ** 16,
+                                                          max_pages=2 ** 10)
+    refused(host, lambda: host.trlm_attn_paged(host.e, c, s, 0x1000, 2 ** 17, 1024, 0.125, 0x2000, 2 ** 17, 0x3000, 2 ** 62),
+            capfd, "trlm_attn_paged")
 
 
 @needs_hip

@@ -39,6 +39,13 @@ __device__ __forceinline__ int paged_seq_of(const int* qs, int n, int row) {
     return lo;
 }
 
+// The tokens sequence seq holds, within [0, 2^30], all that pages can hold: no
+// position formed from it and from rows leaves 32 bits.
+__device__ __forceinline__ int paged_held(const PagedKv& c, int seq) {
+    const int v = c.kv_len[seq];
+    return v < 0 ? 0 : v > 1 << 30 ? 1 << 30 : v;
+}
+
 // The pool row of (sequence, position, head), or -1 where the position has no
 // page.  page_size <= 2^16 and kv_heads <= 2^10: the product is formed in 64 bits.
 __device__ __forceinline__ long long paged_place(const PagedKv& c, int seq, int pos, int head) {
@@ -177,7 +184,7 @@ __device__ __forceinline__ void kv_append(const KvAppendParams& p) {
     int pos = 0;
     long long place = -1;
     if (ok) {
-        pos = p.kv.kv_len[seq] - (qs[seq + 1] - row);
+        pos = paged_held(p.kv, seq) - (qs[seq + 1] - row);
         ok = pos >= 0 && (p.rot == 0 || pos < p.max_pos);
         if (ok) place = paged_place(p.kv, seq, pos, 0);
         ok = ok && place >= 0;
@@ -214,7 +221,7 @@ __device__ __forceinline__ void kv_read(const KvReadParams& p) {
     paged_stage_starts(p.kv, qs);
     const int seq = row < p.kv.rows ? paged_seq_of(qs, p.kv.n, row) : p.kv.n;
     if (seq >= p.kv.n) return;
-    const long long place = paged_place(p.kv, seq, p.kv.kv_len[seq] - (qs[seq + 1] - row), 0);
+    const long long place = paged_place(p.kv, seq, paged_held(p.kv, seq) - (qs[seq + 1] - row), 0);
     f32x4 x[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {

@@ -40,6 +40,12 @@ __device__ __forceinline__ float pa_pow2(int e) {       // 2^e, e kept in [-126,
     return __uint_as_float((unsigned)(e + 127) << 23);
 }
 
+// q_start[i] within the rows (rows x heads is below 2^31, so is what follows from it).
+__device__ __forceinline__ int pa_start(const PagedKv& c, int i) {
+    const int v = c.q_start[i];
+    return v < 0 ? 0 : v > c.rows ? c.rows : v;
+}
+
 // The upper halves of two words, a's below b's: two floats truncated to bf16.
 __device__ __forceinline__ unsigned pa_pack(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
@@ -165,19 +171,15 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
     const int tile = x % tiles;
     x /= tiles;
     const int h = x % c.kv_heads, seq = x / c.kv_heads;
-    int q0 = c.q_start[seq], q1 = c.q_start[seq + 1];
-    const int q1_said = q1;
-    q0 = q0 < 0 ? 0 : q0;
-    q1 = q1 > c.rows ? c.rows : q1;
-    const int qn = q1 - q0 < p.max_q ? q1 - q0 : p.max_q;
+    const int q0 = pa_start(c, seq), q1 = pa_start(c, seq + 1);
+    const int qn = q1 - q0 < 0 ? 0 : q1 - q0 < p.max_q ? q1 - q0 : p.max_q;
     const int R = qn * G, r0 = tile * 16;
     if (r0 >= R || R > p.few_rows) return;
-    const int held = c.kv_len[seq];
-    const int keys = held < 0 ? 0 : held > p.max_kv ? p.max_kv : held;
+    const int held = paged_held(c, seq), keys = held > p.max_kv ? p.max_kv : held;
     const int nr = R - r0 < 16 ? R - r0 : 16;
     // keys that a row may see: [0, lim); first, the row's token
     const int tok = (r0 + (i < nr ? i : nr - 1)) / G, grp = (r0 + (i < nr ? i : nr - 1)) - tok * G;
-    const int pos0 = held - (q1_said - q0);
+    const int pos0 = held - (q1 - q0);
     auto limit = [&](int t) {
         const int l = pos0 + t + 1;
         return l < 0 ? 0 : l > keys ? keys : l;
@@ -542,17 +544,13 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
     const int h = x % c.kv_heads;
     x /= c.kv_heads;
     const int seq = x % c.n, tile = tiles - 1 - x / c.n;
-    int q0 = c.q_start[seq], q1 = c.q_start[seq + 1];
-    const int q1_said = q1;
-    q0 = q0 < 0 ? 0 : q0;
-    q1 = q1 > c.rows ? c.rows : q1;
-    const int qn = q1 - q0 < p.max_q ? q1 - q0 : p.max_q;
+    const int q0 = pa_start(c, seq), q1 = pa_start(c, seq + 1);
+    const int qn = q1 - q0 < 0 ? 0 : q1 - q0 < p.max_q ? q1 - q0 : p.max_q;
     const int R = qn * G, r0 = tile * 32 * NW;
     if (r0 >= R || R <= p.few_rows) return;
-    const int held = c.kv_len[seq];
-    const int keys = held < 0 ? 0 : held > p.max_kv ? p.max_kv : held;
+    const int held = paged_held(c, seq), keys = held > p.max_kv ? p.max_kv : held;
     const int nr = R - r0 < 32 * NW ? R - r0 : 32 * NW;
-    const int pos0 = held - (q1_said - q0);
+    const int pos0 = held - (q1 - q0);
     auto limit = [&](int t) {
         const int l = pos0 + t + 1;
         return l < 0 ? 0 : l > keys ? keys : l;
@@ -1028,15 +1026,14 @@ __device__ __forceinline__ int pa_row_splits(const PagedAttnParams& p, const int
     if (at >= (long long)c.rows * p.heads) return -1;
     const int row = (int)(at / p.heads), seq = paged_seq_of(qs, c.n, row);
     if (seq >= c.n || row - qs[seq] >= p.max_q) return -1;
-    const int held = c.kv_len[seq];
-    const int keys = held < 0 ? 0 : held > p.max_kv ? p.max_kv : held;
-    int qn = c.q_start[seq + 1] - qs[seq];
-    qn = qn < p.max_q ? qn : p.max_q;
+    const int held = paged_held(c, seq), keys = held > p.max_kv ? p.max_kv : held;
+    const int qn = qs[seq + 1] - qs[seq] < p.max_q ? qs[seq + 1] - qs[seq] : p.max_q;
     const int chunk = qn * (p.heads / c.kv_heads) <= p.few_rows ? p.chunk_few : p.chunk_tile;
     if (keys <= chunk) return -1;
-    int lim = held - (c.q_start[seq + 1] - row) + 1;
+    int lim = held - (qs[seq + 1] - row) + 1;
     lim = lim < 0 ? 0 : lim > keys ? keys : lim;
-    return (lim + chunk - 1) / chunk;
+    const int ns = (lim + chunk - 1) / chunk;
+    return ns < p.splits ? ns : p.splits;
 }
 
 // A few splits: HD / 4 lanes a row, 256 / (HD / 4) rows a workgroup.

@@ -285,7 +285,8 @@ static AttnPlan attn_plan(const TrlmKvCache* c, const TrlmKvSeqs* s, u32 heads) 
         p.tiles = (u32)cdiv64(most, TILE_ROWS);
         p.tile_groups = seq_heads * p.tiles;
         p.tile_splits = split_tiles(kv, max_q, p.tile_groups, s->n, &p.chunk_tile);
-        /* one sequence, or as many rows as all sequences at their longest: none is short */
+        /* one sequence, or as many rows as all sequences at their longest: none is short, or should one be
+         * (max_q and rows are bounds), the tile kernel takes it too */
         if (s->n == 1 || (u64)s->n * max_q <= s->rows) p.few_splits = 0;
     }
     p.splits = p.tile_splits > p.few_splits ? p.tile_splits : p.few_splits;
@@ -313,11 +314,14 @@ i32 trlm_attn_paged(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hip
     if (unaligned(q, 16) || unaligned(out, 16) || (ldq | ldo) % 4) return refuse(op, "q and out rows must be 16-byte aligned");
     if (ldq < heads * hd || ldo < heads * hd || (ldq | ldo) > 0x7fffffffu) return refuse(op, "ldq and ldo must hold a row");
     if (!s->n || !s->rows || !s->max_q) return 0;
+    if ((u64)s->rows * heads > 0x7fffffffull) return refuse(op, "rows * heads must be below 2^31");
     const AttnPlan pl = attn_plan(c, s, heads);
     const u64 need = attn_ws(c, s, heads, &pl);
     if (need && (unaligned(ws, 16) || ws_bytes < need)) return refuse(op, "the workspace is too small or not 16-byte aligned");
-    if (pl.few_groups > 0x7fffffffull || pl.tile_groups > 0x7fffffffull || (u64)s->rows * heads > 0x7fffffffull)
-        return refuse(op, "too many workgroups");
+    const int many = pl.splits > JOIN_SPLITS || (u64)s->rows * heads < JOIN_ROWS;
+    const u64 join_groups = pl.splits > 1 ? cdiv64((u64)s->rows * heads, many ? 4 : 1024 / hd) : 0;
+    if (pl.few_groups * 256 > 0xffffffffull || pl.tile_groups * 512 > 0xffffffffull || join_groups * 256 > 0xffffffffull)
+        return refuse(op, "more work than one launch holds (2^32 threads)");
     PagedAttnParams p;
     memset(&p, 0, sizeof(p));
     p.kv = paged_kv(c, s);
@@ -327,7 +331,7 @@ i32 trlm_attn_paged(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hip
     p.ldq = (int)ldq; p.ldo = (int)ldo; p.heads = (int)heads;
     p.max_q = (int)(s->max_q < s->rows ? s->max_q : s->rows);
     p.max_kv = (int)max_kv_of(c, s);
-    p.few_rows = (int)FEW_MAX;
+    p.few_rows = pl.few_splits ? (int)FEW_MAX : 0;
     p.splits = (int)pl.splits; p.chunk_few = (int)pl.chunk_few; p.chunk_tile = (int)pl.chunk_tile;
     p.scale = scale;
     const i32 i = hd_index(hd);
@@ -338,11 +342,9 @@ i32 trlm_attn_paged(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hip
     if (pl.few_splits)
         hip_launch(kernel_hd(e, &e->few[i][c->type], "k_paged_attn_few", i, (i32)c->type), (u32)pl.few_groups,
                    pl.few_splits, 1, 256, 1, 1, 0, args);
-    if (pl.splits > 1) {
-        const int many = pl.splits > JOIN_SPLITS || (u64)s->rows * heads < JOIN_ROWS;
+    if (pl.splits > 1)
         hip_launch(kernel_hd(e, &e->join[i][many], many ? "k_paged_attn_join_long" : "k_paged_attn_join", i, -1),
-                   (u32)cdiv64((u64)s->rows * heads, many ? 4 : 1024 / hd), 1, 1, 256, 1, 1, 0, args);
-    }
+                   (u32)join_groups, 1, 1, 256, 1, 1, 0, args);
     return 0;
 }
 

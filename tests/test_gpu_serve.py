@@ -763,3 +763,73 @@ def test_two_contexts_at_once(trlm, box):
     serve2.close()
     dev2.close()
     dev.current()
+
+
+@pytest.mark.parametrize("type", ALL_TYPES)
+@pytest.mark.parametrize("hd", ALL_HD)
+def test_attn_mixed_batches(trlm, box, type, hd):
+    """Long chunks beside single tokens: row tiles found among the sequences' counts; more of them than the rows with one
+    sequence at its longest suggest (taken in turns); more sequences than a workgroup has threads; long ones anywhere."""
+    rng = np.random.default_rng(71 + hd)
+    attn_case(trlm, box, rng, type, hd, 2, 1, [1, 300, 1, 0, 2, 1], [50, 400, 1, 7, 600, 33], 32, spare_rows=3)
+    attn_case(trlm, box, rng, type, hd, 2, 2, [70] * 6, [90, 70, 200, 70, 71, 300], 16, max_q=420)
+    if hd == 64:
+        attn_case(trlm, box, rng, type, hd, 2, 2, [66] * 20 + [1] * 20, [66] * 20 + [200] * 20, 16, max_q=1340)
+        n = 1100
+        q, kv = np.ones(n, int), rng.integers(1, 40, n)
+        for at, m in ((0, 140), (513, 70), (1025, 65), (1099, 300)):
+            q[at], kv[at] = m, m + 9
+        attn_case(trlm, box, rng, type, hd, 1, 1, q.tolist(), kv.tolist(), 16, spare_rows=1)
+
+
+def test_attn_mixed_batch_captured(trlm, box):
+    """One graph of a mixed batch, replayed with the long sequences elsewhere."""
+    dev, serve = box
+    dev.current()
+    hip = _runtime()
+    rng = np.random.default_rng(73)
+    H, Hkv, hd, page, n = 2, 1, 64, 16, 12
+    seqs = ref.Seqs(rng, [1] * 10 + [300, 90], [320] * n, page)
+    shape = (seqs.num, Hkv, page, hd)
+    pool = ref.Pool("bf16", seqs.num, page, Hkv, hd, rng.standard_normal(shape).astype(np.float32),
+                    rng.standard_normal(shape).astype(np.float32))
+    q = rng.standard_normal((seqs.rows, H * hd)).astype(np.float32)
+    cache, s = pool.upload(dev, trlm), seqs.upload(dev, trlm)
+    d_q, d_o = dev.upload(q), dev.upload(q)
+    ws_bytes = serve.attn_workspace(cache, s, H)
+    ws = dev.empty(ws_bytes)
+
+    def step():
+        serve.attn(cache, s, d_q, H * hd, H, 0.125, d_o, H * hd, ws, ws_bytes)
+
+    step()
+    dev.sync()
+    stream, graph, exe = C.c_void_p(dev.ctx.stream), C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 2) == 0
+    step()
+    assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)) == 0
+    try:
+        for lens in ([1] * 10 + [300, 90], [65] * 6 + [1] * 6, [0, 200, 1, 70, 0, 0, 120, 9, 0, 0, 0, 0], [1] * n):
+            seqs.q_len, seqs.kv_len = lens, [m + int(rng.integers(0, 20)) for m in lens]
+            seqs.q_start = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+            for p, a in ((seqs.ptr[0], seqs.q_start), (seqs.ptr[1], np.array(seqs.kv_len, np.int32))):
+                dev.hip.hip_h2d(p, a.ctypes.data, a.nbytes)
+            want, bound = ref.attention(pool, seqs, q, H, 0.125)
+            outs = []
+            for eager in (False, True, False):
+                dev.hip.hip_h2d(d_o, q.ctypes.data, q.nbytes)
+                if eager:
+                    step()
+                else:
+                    assert hip.hipGraphLaunch(exe, stream) == 0
+                dev.sync()
+                outs.append(dev.download(d_o, q.shape))
+            assert same(outs[0], outs[1]) and same(outs[2], outs[1])
+            used = int(seqs.q_start[-1])
+            assert np.array_equal(outs[0][used:], q[used:])
+            err = np.abs(outs[0][:used].reshape(used, H, hd) - want[:used])
+            assert np.all(err <= bound[:used][..., None])
+    finally:
+        hip.hipGraphExecDestroy(exe)
+        hip.hipGraphDestroy(graph)

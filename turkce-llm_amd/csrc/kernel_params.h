@@ -135,6 +135,7 @@ typedef struct PagedAttnParams {
     int ldq, ldo, heads;
     int max_q, max_kv;
     int few_rows;            // sequences of at most so many rows (tokens x group) go to the few-rows kernel
+    int few_apart;           // the few-rows kernel's grid: all sequences' first tiles first
     int splits;              // slots of a row's parts
     int chunk_few, chunk_tile;   // keys [s * chunk, (s + 1) * chunk) of a sequence are split s
     float scale;

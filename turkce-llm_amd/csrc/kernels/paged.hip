@@ -161,6 +161,9 @@ __device__ __forceinline__ void paged_store(void* pool, float* scales, long long
 // row's numbers of a head are read as one run, consecutive tokens of a sequence
 // write consecutive cache rows, and a row's place and angles are found once for
 // its U heads.  All U loads are in flight before the first use.
+// Bound by the memory for prompts: 8 x 1024 tokens, 32 + 2 x 8 heads of 128, 8 bits, with
+// their read back: 102 us, 441 MB at 4.3 TB/s (a copy: 4.9).  By the launch for
+// single tokens: 64 of 6 + 2 x 6 heads of 64 3.7 us.
 template <int HD, int TYPE, int U>
 __device__ __forceinline__ void kv_append(const KvAppendParams& p) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR;
@@ -210,7 +213,7 @@ __device__ __forceinline__ void kv_append(const KvAppendParams& p) {
 
 // ------------------------------------------------------------------ read
 // The inverse, in the same order: blockIdx.y over the key heads, then the value
-// heads.
+// heads.  Bound by the memory: 16 sequences in bf16 497 MB, 120 us, 4.1 TB/s.
 template <int HD, int TYPE, int U>
 __device__ __forceinline__ void kv_read(const KvReadParams& p) {
     constexpr int LPR = HD / 4, RPB = 256 / LPR;

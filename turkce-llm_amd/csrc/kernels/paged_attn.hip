@@ -3,13 +3,14 @@
 //   out[i] = sum_{t <= pos(i)} w_t v_t / sum w_t,   w_t = 2^(s_t - m),
 //   s_t = <q_i, k_t> scale log2(e),  m = max s_t    (online over key blocks)
 //
-// Products on the bf16 matrix cores without loss of fp32 precision: a number
-// x of fp32 is the exact sum of three bf16 numbers (its mantissa's upper,
-// middle and lower 8 bits, by truncation, so nothing overflows), a bf16 or
-// 8-bit cached number is one bf16 number exactly.  A product of two fp32
-// numbers takes the six of its nine partial products that reach 24 bits, one
-// with a cached bf16 or 8-bit number three, all exact; sums are fp32.  An
-// 8-bit key's scale multiplies its score, an 8-bit value's scale its weight.
+// Products keep fp32's precision on the 16-bit matrix cores.  Few rows (paged_attn_few),
+// fp32 and bf16 caches: a number of fp32 is the exact sum of three bf16 numbers
+// (its mantissa's upper, middle and lower 8 bits, by truncation, so nothing
+// overflows), a bf16 number one; a product of two fp32 numbers takes the six of
+// its nine partial products that reach 24 bits, one with a bf16 number three.
+// 8-bit caches, and all caches in the many-rows kernel, where the products and
+// not the memory bound: two f16 terms and exact powers of two, below.  Sums are
+// fp32.  An 8-bit key's scale multiplies its score, an 8-bit value's its weight.
 //
 // A head's queries: with G query heads to a cached head, rows r = token * G +
 // (head in its group) of one cached head are computed together, so its keys
@@ -27,11 +28,10 @@ typedef unsigned pa_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned pa_u32x2 __attribute__((ext_vector_type(2)));
 
 #define PA_EXP_MIN 12      // rows below 2^-115 take the power of 2^-115 (their scale is then 2^126)
-#define PA_W 10            // a row's weights go up to 2^10, ..
+#define PA_W 10            // a row's weights go up to 2^10, and to 2^14 while its maximum grows (PA_GROW)
 #define PA_UP 11           // a row's largest magnitude goes to about 2^11 ..
 #define PA_ABOVE 3         // .. and may be up to 2^3 above that
 #define PA_BELOW 6         // .. or 2^6 below; together below f16's 2^16
-#define PA_I8_UP 0         // 8-bit integers stay themselves
 #define PA_FEW_W 13        // the few-rows kernel's weights (8 bits) go up to 2^14
 #define PA_GROW 4.0f       // a row's maximum may grow by so much (weights to 2^PA_W 2^4) before its sums are rescaled
 
@@ -154,6 +154,12 @@ struct PaRun {
 //     HD / 16 + e, one product for each e.
 // A row (query) is one lane column throughout, so its maximum and rescaling
 // need two exchanges (lanes 16 and 32 away) and no broadcast.
+// Bound by the memory where the contexts are long: 32 single tokens over up to
+// 8192, 8 bits, 32 heads on 8 of 128: 69 us with their join, 265 MB at 3.9 TB/s (three bf16
+// terms for 8 bits too: 95; keys read a block ahead: no gain, the workgroups of
+// a unit hide one another's loads); 64 over up to 1024, fp32, 6 heads of 64: 24 us
+// and 5 of join, 110 MB.  By the latency of its two launches where they are
+// short: one token over 1000 9.5 us.
 template <int HD, int TYPE>
 __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
     constexpr int KD = HD / 4, VD = HD / 16, NS = (KD + 7) / 8;
@@ -165,12 +171,16 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, kq = lane >> 4;
     const int G = p.heads / c.kv_heads;
+    // A sequence's tiles next to one another; in a mixed batch, where most
+    // sequences have one tile of the grid's four, all first tiles first (next to
+    // one another those with work would be on every fourth place and so on few
+    // of the units: one prompt of 1024 and 256 single tokens over 500, head_dim
+    // 128, 340 us against 169).
     const int most = p.max_q * G < p.few_rows ? p.max_q * G : p.few_rows;
-    const int tiles = (most + 15) >> 4;
-    int x = blockIdx.x;
-    const int tile = x % tiles;
-    x /= tiles;
-    const int h = x % c.kv_heads, seq = x / c.kv_heads;
+    const int tiles = (most + 15) >> 4, pairs = c.n * c.kv_heads;
+    const int tile = p.few_apart ? blockIdx.x / pairs : blockIdx.x % tiles;
+    const int pair = p.few_apart ? blockIdx.x % pairs : blockIdx.x / tiles;
+    const int h = pair % c.kv_heads, seq = pair / c.kv_heads;
     const int q0 = pa_start(c, seq), q1 = pa_start(c, seq + 1);
     const int qn = q1 - q0 < 0 ? 0 : q1 - q0 < p.max_q ? q1 - q0 : p.max_q;
     const int R = qn * G, r0 = tile * 16;
@@ -489,8 +499,10 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
 //     their rows' largest magnitudes into [2^5, 2^15) (two terms are good to
 //     22 bits of a number and to 2^-25: 30 bits of its row's largest at least);
 //   with V' = 2^-ev V a second running maximum mo is kept, of s + ev: weights
-//     2^(s + ev - mo + 14) <= 2^14 are small against the largest contribution to
-//     the row, not against the largest weight; their sum is taken back to m.
+//     2^(s + ev - mo + 10) are small against the largest contribution to the
+//     row, not against the largest weight; their sum is taken back to m.  Both
+//     maxima are followed only when a row outgrows its own by 2^4 (weights to
+//     2^14), which saves most rescalings.
 // The powers of a tile are those of the tile before it.  A tile whose rows do
 // not fit them (the first one, or rows of very different magnitude next to one
 // another) is taken again by classes of keys that fit one pair of powers,
@@ -501,6 +513,12 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
 // S^T = K Q^T puts a row into a lane's column, as in attention.hip, and the
 // exponentiated result is operand B of O^T += V^T P^T as it is: registers 8 u
 // .. 8 u + 7 of lane half h are the keys 16 u + 8 a + 4 h + c (a < 2, c < 4).
+// Bound by the matrix cores and, beside them, the exponentials' VALU work: 2048
+// tokens over 16384 in bf16, 32 heads on 8 of 128: 1.1 ms, 465 TF/s of the
+// mathematics and 930 of f16 products (a large f16 product: 1149); 8 prompts of
+// 1024, fp32, 6 heads of 64: 46 us and 4 of join, a unit's 8 tiles at 4.5 us and its
+// start.  256 rows (eight waves of 32) share each staged tile: 128 rows in four
+// waves, two workgroups a unit, staged everything twice and were slower.
 // V^T is read from V's own rows by ds_read_b64_tr_b16: of 16 lanes, lanes 4 e ..
 // 4 e + 3 address 16 numbers of row e, and lane j receives number j of rows 0 .. 3.
 typedef unsigned short pa_u16x2 __attribute__((ext_vector_type(2)));
@@ -523,8 +541,17 @@ __device__ __forceinline__ int pa_wave_max(int v) {
     return v;
 }
 
+// Row tiles of a sequence in this kernel: none where the few-rows kernel takes it.
+template <int NW>
+__device__ __forceinline__ int pa_tiles_of(const PagedAttnParams& p, int seq) {
+    const int q = pa_start(p.kv, seq + 1) - pa_start(p.kv, seq);
+    const int R = (q < 0 ? 0 : q < p.max_q ? q : p.max_q) * (p.heads / p.kv.kv_heads);
+    return R <= p.few_rows ? 0 : (R + 32 * NW - 1) / (32 * NW);
+}
+
+// One row tile of one sequence and head.
 template <int HD, int TYPE, int NW, int KB>
-__device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
+__device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p, int h, int seq, int tile, int (&kbad)[64]) {
     constexpr int THREADS = 64 * NW, NT = TYPE == KV_F32 ? 2 : 1;
     constexpr int CPR = HD / 8, CH = KB * CPR, CK = (CH + THREADS - 1) / THREADS;   // 8-number chunks
     constexpr int NS = HD / 16, DB = (HD + 31) / 32, KT = KB / 32;
@@ -533,17 +560,11 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
     constexpr int KTERM = KB * KLD, VTERM = KB * HD * 2, BUF = NT * (KTERM + VTERM);
     __shared__ __attribute__((aligned(16))) char tbuf[2 * BUF];   // two buffers of K terms, then V terms
     __shared__ __attribute__((aligned(16))) float ksc[TYPE == KV_I8 ? 2 : 1][KB], vsc[TYPE == KV_I8 ? 2 : 1][KB];
-    __shared__ int misfit[2], kbad[64], lek[KB], lev[KB];
+    __shared__ int misfit[2], lek[KB], lev[KB];
     __shared__ __attribute__((aligned(16))) int bad[HD];
     const PagedKv& c = p.kv;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int G = p.heads / c.kv_heads;
-    const int tiles = (p.max_q * G + 32 * NW - 1) / (32 * NW);
-    // the last rows (which see the most keys) first
-    int x = blockIdx.x;
-    const int h = x % c.kv_heads;
-    x /= c.kv_heads;
-    const int seq = x % c.n, tile = tiles - 1 - x / c.n;
     const int q0 = pa_start(c, seq), q1 = pa_start(c, seq + 1);
     const int qn = q1 - q0 < 0 ? 0 : q1 - q0 < p.max_q ? q1 - q0 : p.max_q;
     const int R = qn * G, r0 = tile * 32 * NW;
@@ -761,8 +782,8 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
         const int i = lane & 15, p_ = CPR >= 8 ? (i >> 2) & 1 : 0;
         const int dims = (16 * ((lane >> 4) & 1) + 4 * (i & 3)) & (HD - 1);
         const char* vt = tbuf + buf * BUF + NT * KTERM + (4 * half + (i >> 2)) * HD * 2 + dims * 2;
-        const float cu = pa_pow2(qe + (TYPE == KV_I8 ? -PA_I8_UP : EK - 127 - PA_UP));
-        const float ev = (float)(EV - 127 - (TYPE == KV_I8 ? PA_I8_UP : PA_UP));
+        const float cu = pa_pow2(qe + (TYPE == KV_I8 ? 0 : EK - 127 - PA_UP));
+        const float ev = (float)(EV - 127 - (TYPE == KV_I8 ? 0 : PA_UP));
         float minus = -1.0f;
         asm("" : "+s"(minus));      // kept a factor: v_fma_mix takes the f16 term as it is
         auto scores = [&](int t, f32x16& s) {
@@ -1014,6 +1035,68 @@ __device__ __forceinline__ void paged_attn_tile(const PagedAttnParams& p) {
     }
 }
 
+// Where all sequences may be as long as the longest (or there is one) the grid
+// holds max_q's tiles of each, the last rows, which see the most keys, first.
+template <int HD, int TYPE, int NW, int KB>
+__device__ __forceinline__ void paged_attn_tile_dense(const PagedAttnParams& p) {
+    __shared__ int kbad[64];
+    const int tiles = (p.max_q * (p.heads / p.kv.kv_heads) + 32 * NW - 1) / (32 * NW);
+    const int x = blockIdx.x / p.kv.kv_heads;
+    paged_attn_tile<HD, TYPE, NW, KB>(p, blockIdx.x % p.kv.kv_heads, x % p.kv.n, tiles - 1 - x / p.kv.n, kbad);
+}
+
+// In a mixed batch that would be mostly workgroups without work, each a compute
+// unit's turn (a prompt of 2048 beside 64 single tokens 204 us, so 94).  There
+// the grid holds the tiles that the call's rows make up with
+// one sequence at its longest, and a workgroup finds its own among the sequences'
+// counts, which its threads add up together; should there be more tiles, the
+// workgroups take them in turns.
+template <int HD, int TYPE, int NW, int KB>
+__device__ __forceinline__ void paged_attn_tile_mixed(const PagedAttnParams& p) {
+    const PagedKv& c = p.kv;
+    __shared__ int few[64];
+    const int h = blockIdx.x % c.kv_heads;
+    int j = blockIdx.x / c.kv_heads, more;
+    do {
+        const int per = (c.n + 64 * NW - 1) / (64 * NW);
+        const int s0 = threadIdx.x * per, s1 = s0 + per < c.n ? s0 + per : c.n;
+        int own = 0;
+        for (int s = s0; s < s1; s++) own += pa_tiles_of<NW>(p, s);
+        int upto = own;                                // tiles up to this thread's last sequence
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(upto, o, WAVE);
+            if ((int)(threadIdx.x & 63) >= o) upto += v;
+        }
+        if ((threadIdx.x & 63) == 63) few[threadIdx.x >> 6] = upto;
+        __syncthreads();
+        int total = 0;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const int v = few[w];
+            if (w < (int)(threadIdx.x >> 6)) upto += v;
+            total += v;
+        }
+        if (j >= total) return;                        // the same for all threads
+        if (j < upto && j >= upto - own) {
+            int left = upto - j, s = s1 - 1, n = pa_tiles_of<NW>(p, s);
+            while (left > n) {
+                left -= n;
+                n = pa_tiles_of<NW>(p, --s);
+            }
+            few[NW] = s;
+            few[NW + 1] = left - 1;
+        }
+        __syncthreads();
+        const int seq = __builtin_amdgcn_readfirstlane(few[NW]), tile = __builtin_amdgcn_readfirstlane(few[NW + 1]);
+        j += gridDim.x / c.kv_heads;
+        more = __builtin_amdgcn_readfirstlane(total) - j;
+        __syncthreads();
+        paged_attn_tile<HD, TYPE, NW, KB>(p, h, seq, tile, few);
+        __syncthreads();
+    } while (more > 0);
+}
+
 // ------------------------------------------------------------------ join
 // out = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over a row's splits, in
 // one order.  Sequences of one split are finished already.
@@ -1113,12 +1196,16 @@ __device__ __forceinline__ void paged_attn_join_long(const PagedAttnParams& p) {
     if (g == 0) *(f32x4*)(p.out + at / p.heads * p.ldo + at % p.heads * HD + d) = a;
 }
 
+#define PA_KEYS(HD, TYPE) (HD == 128 && TYPE == KV_F32 ? 32 : 64)      // of a stage
 #define PA_KERNELS(HD, NAME, TYPE)                                                                              \
     extern "C" __global__ void __launch_bounds__(256) k_paged_attn_few_hd##HD##_##NAME(PagedAttnParams p) {     \
         paged_attn_few<HD, TYPE>(p);                                                                            \
     }                                                                                                           \
     extern "C" __global__ void __launch_bounds__(512, 2) k_paged_attn_tile_hd##HD##_##NAME(PagedAttnParams p) { \
-        paged_attn_tile<HD, TYPE, 8, HD == 128 && TYPE == KV_F32 ? 32 : 64>(p);                                                                    \
+        paged_attn_tile_dense<HD, TYPE, 8, PA_KEYS(HD, TYPE)>(p);                                               \
+    }                                                                                                           \
+    extern "C" __global__ void __launch_bounds__(512, 2) k_paged_attn_mixed_hd##HD##_##NAME(PagedAttnParams p) { \
+        paged_attn_tile_mixed<HD, TYPE, 8, PA_KEYS(HD, TYPE)>(p);                                               \
     }
 #define PA_TYPES(HD)                                                                                            \
     PA_KERNELS(HD, f32, KV_F32)                                                                                 \

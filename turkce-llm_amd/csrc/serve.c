@@ -18,7 +18,7 @@ struct TrlmServe {
     HipCtx* ctx;
     i32 device;
     /* looked up on first use of a head width and type */
-    hipFunction_t append[NHD][NTYPE][2], read[NHD][NTYPE][2], few[NHD][NTYPE], tile[NHD][NTYPE], join[NHD][2];
+    hipFunction_t append[NHD][NTYPE][2], read[NHD][NTYPE][2], few[NHD][NTYPE], tile[NHD][NTYPE][2], join[NHD][2];
     hipFunction_t rules[2][2];   /* [narrow, wide][aligned, not] */
 };
 
@@ -206,6 +206,12 @@ i32 trlm_kv_read(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hipDev
 #define FEW_MAX 64u
 #define TILE_ROWS 256u    /* rows of a k_paged_attn_tile workgroup: its registers fill a compute unit */
 #define TILE_KEYS 64u     /* keys of its stages */
+/* The kernel that looks its tile up (and spills registers at head_dim 128, 15%)
+ * is taken where the tiles that a call's rows make up are less than half of all
+ * sequences' at their longest.  Measured, with and without: a prompt of 2048
+ * beside 64 single tokens over 1000 94 / 204 us; 8 prompts of 90 to 2000 (28 of
+ * 64 tiles) 66 / 93; 64 of 70 to 300 (110 of 128) 57 / 56. */
+#define MIXED_MIN 2u
 #define CUS 256u
 #define MAX_SPLITS 256u
 
@@ -213,6 +219,8 @@ typedef struct AttnPlan {
     u32 few_tiles, tiles;             /* row tiles of a sequence in each kernel (0: not launched) */
     u32 few_splits, tile_splits, chunk_few, chunk_tile, splits;
     u64 few_groups, tile_groups;
+    int few_apart;
+    int mixed;                        /* tile_groups: what the rows make up, not the longest's for each */
 } AttnPlan;
 
 static u32 max_kv_of(const TrlmKvCache* c, const TrlmKvSeqs* s) {
@@ -275,7 +283,14 @@ static AttnPlan attn_plan(const TrlmKvCache* c, const TrlmKvSeqs* s, u32 heads) 
     const u64 most = (u64)max_q * group, seq_heads = (u64)s->n * c->kv_heads;
     p.few_tiles = (u32)cdiv64(most < FEW_MAX ? most : FEW_MAX, FEW_TILE);
     p.few_groups = seq_heads * p.few_tiles;
-    p.few_splits = split_keys(kv, p.few_groups, FEW_GROUPS, FEW_KEYS, &p.chunk_few);
+    /* rest: of the rows, what one sequence at its longest leaves; busy: the row tiles that may have work.  Where
+     * they are at most half of the grid, as in calls that mix long and short sequences, the others are kept apart
+     * and the splits planned without them (16 sequences of 1 .. 8 tokens, nearly all tiles busy: 38 us, apart 44). */
+    const u64 rest = ((u64)s->rows - max_q) * group, few_all = (u64)s->n * p.few_tiles;
+    u64 busy = s->n + rest / FEW_TILE;
+    p.few_apart = most > FEW_MAX || 2 * busy <= few_all;
+    if (!p.few_apart || busy > few_all) busy = few_all;
+    p.few_splits = split_keys(kv, busy * c->kv_heads, FEW_GROUPS, FEW_KEYS, &p.chunk_few);
     if (kv <= FEW_WHOLE) {
         p.few_splits = 1;
         p.chunk_few = (u32)(cdiv64(kv, FEW_KEYS) * FEW_KEYS);
@@ -283,8 +298,13 @@ static AttnPlan attn_plan(const TrlmKvCache* c, const TrlmKvSeqs* s, u32 heads) 
     p.chunk_tile = p.chunk_few;
     if (most > FEW_MAX) {
         p.tiles = (u32)cdiv64(most, TILE_ROWS);
-        p.tile_groups = seq_heads * p.tiles;
-        p.tile_splits = split_tiles(kv, max_q, p.tile_groups, s->n, &p.chunk_tile);
+        const u64 all = (u64)s->n * p.tiles;
+        u64 t = p.tiles + (s->n - 1 < rest / FEW_MAX ? s->n - 1 : rest / FEW_MAX) + rest / TILE_ROWS;
+        if (t > all) t = all;
+        p.mixed = t * MIXED_MIN < all;
+        if (!p.mixed) t = all;
+        p.tile_groups = t * c->kv_heads;
+        p.tile_splits = split_tiles(kv, max_q, t * c->kv_heads, s->n, &p.chunk_tile);
         /* one sequence, or as many rows as all sequences at their longest: none is short, or should one be
          * (max_q and rows are bounds), the tile kernel takes it too */
         if (s->n == 1 || (u64)s->n * max_q <= s->rows) p.few_splits = 0;
@@ -332,12 +352,14 @@ i32 trlm_attn_paged(TrlmServe* e, const TrlmKvCache* c, const TrlmKvSeqs* s, hip
     p.max_q = (int)(s->max_q < s->rows ? s->max_q : s->rows);
     p.max_kv = (int)max_kv_of(c, s);
     p.few_rows = pl.few_splits ? (int)FEW_MAX : 0;
+    p.few_apart = pl.few_apart;
     p.splits = (int)pl.splits; p.chunk_few = (int)pl.chunk_few; p.chunk_tile = (int)pl.chunk_tile;
     p.scale = scale;
     const i32 i = hd_index(hd);
     void* args[] = { &p };
     if (pl.tiles)
-        hip_launch(kernel_hd(e, &e->tile[i][c->type], "k_paged_attn_tile", i, (i32)c->type), (u32)pl.tile_groups,
+        hip_launch(kernel_hd(e, &e->tile[i][c->type][pl.mixed], pl.mixed ? "k_paged_attn_mixed" : "k_paged_attn_tile", i,
+                             (i32)c->type), (u32)pl.tile_groups,
                    pl.tile_splits, 1, 512, 1, 1, 0, args);
     if (pl.few_splits)
         hip_launch(kernel_hd(e, &e->few[i][c->type], "k_paged_attn_few", i, (i32)c->type), (u32)pl.few_groups,

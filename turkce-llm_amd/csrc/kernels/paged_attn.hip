@@ -513,9 +513,10 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnParams& p) {
 // S^T = K Q^T puts a row into a lane's column, as in attention.hip, and the
 // exponentiated result is operand B of O^T += V^T P^T as it is: registers 8 u
 // .. 8 u + 7 of lane half h are the keys 16 u + 8 a + 4 h + c (a < 2, c < 4).
-// Bound by the matrix cores and, beside them, the exponentials' VALU work: 2048
-// tokens over 16384 in bf16, 32 heads on 8 of 128: 1.1 ms, 465 TF/s of the
-// mathematics and 930 of f16 products (a large f16 product: 1149); 8 prompts of
+// Bound by the matrix products and the exponentials' VALU work (38% and about
+// half of the cycles) of the two waves that a SIMD's registers hold, which
+// overlap in part: 2048 tokens over 16384 in bf16, 32 heads on 8 of 128: 1.1 ms, 465
+// TF/s of the mathematics and 930 of f16 products (a large f16 product: 1149); 8 prompts of
 // 1024, fp32, 6 heads of 64: 46 us and 4 of join, a unit's 8 tiles at 4.5 us and its
 // start.  256 rows (eight waves of 32) share each staged tile: 128 rows in four
 // waves, two workgroups a unit, staged everything twice and were slower.

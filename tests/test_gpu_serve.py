@@ -614,6 +614,13 @@ def test_attn_bounds_wider_than_the_call(trlm, box, type, q_len, kv_len, spare, 
 
 
 @pytest.mark.parametrize("type", ALL_TYPES)
+@pytest.mark.parametrize("q_len,kv_len", [([300], [100]), ([400, 1, 200], [30, 9, 0])])
+def test_attn_more_new_tokens_than_kept(trlm, box, type, q_len, kv_len):
+    """The first of them see nothing, and the plan does not count on them."""
+    attn_case(trlm, box, np.random.default_rng(49), type, 64, 4, 2, q_len, kv_len, 32)
+
+
+@pytest.mark.parametrize("type", ALL_TYPES)
 @pytest.mark.parametrize("page", [16, 65536])
 def test_page_sizes_at_the_ends(trlm, box, type, page):
     rng = np.random.default_rng(53)

@@ -12,10 +12,10 @@
  * not kept to fp32.
  *
  * Six layers of d_model 384, V 31769, all sequences past 256 tokens, one token
- * each with its greedy pick (host calls included): 1 sequence 355 us, 16
- * sequences 383, 64 sequences 431 with a bf16 cache (fp32 475, int8 431); the
- * fixed batch of gpu_decode.c, whose step is fused for equal lengths, 269, 293
- * and 309.  Both wait on launches and small products, not on the cache.
+ * each with its greedy pick (host calls included): 1 sequence 350 us, 16
+ * sequences 381, 64 sequences 447 with a bf16 cache (fp32 490, int8 442); the
+ * fixed batch of gpu_decode.c, whose step is fused for equal lengths, 268, 293
+ * and 308.  Both wait on launches and small products, not on the cache.
  */
 #include <stdio.h>
 #include <stdlib.h>
@@ -310,7 +310,8 @@ i32 gpu_paged_extend(TrlmPagedDecoder* d, u32 n, const u32* seqs, const u32* len
         if (s->len + lens[i] > max_kv) max_kv = s->len + lens[i];
     }
     free(seen);
-    if (!why && R >= (1u << 24)) why = "2^24 rows or more";
+    if (!why && (R >= (1u << 24) || R * d->g->H >= (1ull << 31) || (u64)n * d->g->H >= (1u << 22)))
+        why = "more rows or sequences than one call of the operators takes";
     for (u64 r = 0; r < R && !why; r++)
         if (ids[r] >= d->g->V) why = "a token outside the vocabulary";
     if (!why && want > d->num_free) why = "no pages left";

@@ -8,7 +8,7 @@
 // re-read by every slice of its row, from the L2.
 // Bound by the memory where the rows are many: 256 rows of 131072 269 MB, 56 us,
 // 4.8 TB/s (a copy: 4.9).  64 rows of 31769 with 1024 tokens of history 6.6 us, one
-// row 4.3: the launch, and the history's dependent reads.
+// row 4.8: the launch, and the history's dependent reads.
 #include "common.h"
 #include "../kernel_params.h"
 

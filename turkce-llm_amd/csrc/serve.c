@@ -250,6 +250,7 @@ static u32 split_keys(u32 kv, u64 groups, u32 wanted, u32 unit, u32* chunk) {
 static u32 split_tiles(u32 kv, u32 max_q, u64 groups, u32 n, u32* chunk) {
     u64 best = 0;
     u32 best_s = 1;
+    if (max_q > kv) max_q = kv;       /* more new tokens than kept ones: the first see nothing */
     *chunk = (u32)(cdiv64(kv, TILE_KEYS) * TILE_KEYS);
     for (u32 s = 1; s <= MAX_SPLITS && (s == 1 || s * groups <= 4 * CUS); s++) {
         const u32 c = (u32)(cdiv64(cdiv64(kv, s), TILE_KEYS) * TILE_KEYS);

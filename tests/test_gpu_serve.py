@@ -840,3 +840,39 @@ def test_attn_mixed_batch_captured(trlm, box):
     finally:
         hip.hipGraphExecDestroy(exe)
         hip.hipGraphDestroy(graph)
+
+
+def test_first_call_of_a_handle_captured(trlm, box):
+    """A handle finds its kernels at their first use, which may be inside a capture."""
+    dev, _ = box
+    dev.current()
+    serve = trlm.Serve(dev)
+    hip = _runtime()
+    rng = np.random.default_rng(79)
+    H, Hkv, hd, page = 2, 1, 32, 16
+    seqs = ref.Seqs(rng, [1, 80], [700, 90], page)
+    shape = (seqs.num, Hkv, page, hd)
+    pool = ref.Pool("i8", seqs.num, page, Hkv, hd, rng.standard_normal(shape).astype(np.float32),
+                    rng.standard_normal(shape).astype(np.float32))
+    q = rng.standard_normal((seqs.rows, H * hd)).astype(np.float32)
+    cache, s = pool.upload(dev, trlm), seqs.upload(dev, trlm)
+    d_q, d_o = dev.upload(q), dev.empty(q.nbytes)
+    ws_bytes = serve.attn_workspace(cache, s, H)
+    ws = dev.empty(ws_bytes)
+    dev.sync()
+    stream, graph, exe = C.c_void_p(dev.ctx.stream), C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 2) == 0
+    serve.attn(cache, s, d_q, H * hd, H, 0.2, d_o, H * hd, ws, ws_bytes)
+    assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)) == 0
+    want, bound = ref.attention(pool, seqs, q, H, 0.2)
+    try:
+        for _ in range(3):
+            assert hip.hipGraphLaunch(exe, stream) == 0
+            dev.sync()
+            got = dev.download(d_o, q.shape).reshape(-1, H, hd)
+            assert np.all(np.abs(got - want) <= bound[..., None])
+    finally:
+        hip.hipGraphExecDestroy(exe)
+        hip.hipGraphDestroy(graph)
+        serve.close()
